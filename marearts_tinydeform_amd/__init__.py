@@ -12,11 +12,14 @@ import operator
 import torch
 
 from . import _native
-from .reference import layer_locations_reference, ma_deform_attn_layer_reference, ma_deform_attn_reference
+from .dense import ma_attn, ma_attn_train, ma_layer_norm, ma_layer_norm_train
+from .reference import (layer_locations_reference, ma_attn_reference, ma_deform_attn_layer_reference,
+                        ma_deform_attn_reference, ma_layer_norm_reference)
 
 __all__ = ['ma_deform_attn', 'ma_deform_attn_reference', 'choose_mode', 'ma_deform_sample', 'ma_deform_sample_v2',
            'predict_us', 'cost_features', 'gap_features', 'ma_deform_attn_layer', 'ma_deform_attn_layer_reference', 'layer_locations_reference',
-           'MSDeformAttnLayer', 'ma_deform_attn_train', 'ma_deform_sample_train']
+           'MSDeformAttnLayer', 'ma_deform_attn_train', 'ma_deform_sample_train', 'ma_attn', 'ma_attn_train',
+           'ma_attn_reference', 'ma_layer_norm', 'ma_layer_norm_train', 'ma_layer_norm_reference']
 __version__ = '0.1.1'  # the version of the reference API this package implements (marearts_tinydeform 0.1.1)
 
 MODES = ('auto', 'fused', 'project')

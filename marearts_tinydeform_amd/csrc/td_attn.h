@@ -1,0 +1,39 @@
+// Attention among tokens: what the forward and backward kernels share (td_attn.hip, td_attn_forward.hip,
+// td_attn_backward.hip).
+#pragma once
+
+#include "../../include/tinydeform_dense.h"
+#include "td_internal.h"
+
+namespace td {
+
+// Heads that share a key head are rows of one problem: row r of (batch b, key head hk) is query r / G of head
+// hk * G + r % G, so that a tile of rows reads each key once and the key gradients of shared heads are one sum.
+struct AttnParams {
+    const void *q, *k, *v, *mask;
+    const uint8_t* pad;
+    void *out, *stats;
+    int64_t qs[3], ks[3], vs[3], ms[3];  // batch, token (query), head strides in elements
+    int B, Q, K, H, Hk, D, G;
+    int rows;       // Q * G
+    FastDiv gdiv;   // r / G
+    int mask_type;  // TD_MASK_*
+    int causal;
+    int64_t diag;   // K - Q: with causal, query i sees the keys j <= i + diag
+    double scale;
+    float c;        // scale * log2(e): scores in base 2
+    // backward
+    const void* go;
+    void *dq, *dk, *dv;
+    void* delta;    // [B, H, Q] in the accumulation type: grad_out . out
+    // workspace of the forward's key split, of the backward
+    void* ws;
+};
+
+AttnParams attn_params(const td_attn_args& a);
+
+// Every launcher returns 0 or a negative TD_E* code after recording a message.
+int launch_attn_forward_generic(int dtype, const AttnParams& p, hipStream_t stream);
+int launch_attn_backward_generic(int dtype, const AttnParams& p, hipStream_t stream);
+
+}  // namespace td

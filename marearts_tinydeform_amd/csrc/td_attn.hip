@@ -1,0 +1,357 @@
+// Attention among tokens (include/tinydeform_dense.h): the argument checks of its C entries, and kernels for any type,
+// head width and stride, one wavefront a row, on the vector units.
+#include <math.h>
+
+#include "td_attn.h"
+
+namespace td {
+namespace {
+
+template <typename T>
+__device__ __forceinline__ const T* at(const void* base, const int64_t (&s)[3], int b, int tok, int h) {
+    return static_cast<const T*>(base) + b * s[0] + static_cast<int64_t>(tok) * s[1] + h * s[2];
+}
+
+template <typename A>
+constexpr A neg_inf() {
+    return -static_cast<A>(__builtin_inf());
+}
+
+// Whether (query i, key j) is left out by causal, padding or the mask, and the additive mask's term. A -inf of a float
+// mask leaves the pair out whatever its score is.
+template <typename T, typename A>
+__device__ __forceinline__ bool pair_masked(const AttnParams& p, int b, int h, int i, int j, A& add) {
+    add = static_cast<A>(0);
+    if (p.causal && j > i + p.diag) return true;
+    if (p.pad != nullptr && p.pad[static_cast<int64_t>(b) * p.K + j]) return true;
+    if (p.mask_type == TD_MASK_NONE) return false;
+    const int64_t m = b * p.ms[0] + h * p.ms[1] + i * p.ms[2] + j;
+    if (p.mask_type == TD_MASK_BYTES) return static_cast<const uint8_t*>(p.mask)[m] != 0;
+    add = cvt<A>(static_cast<const T*>(p.mask)[m]);
+    return add == neg_inf<A>();
+}
+
+template <typename A>
+__device__ __forceinline__ A wave_max(A v) {
+#pragma unroll
+    for (int m = 32; m > 0; m >>= 1) {
+        const A o = xor_lane(v, m);
+        v = o > v ? o : v;
+    }
+    return v;
+}
+
+constexpr int kMaxPerLane = TD_ATTN_MAX_HEAD_DIM / kWave;  // head channels per lane
+
+// One wavefront per (b, h, i): keys 64 at a time, one per lane for the scores, then lanes over the head's channels.
+// The running maximum m and sum l (Milakov and Gimelshein's one-pass softmax) are kept in the accumulation type. Bound by
+// the latency of its row loads; the matrix-unit kernels take every case in 16 and 32 bits that they can.
+template <typename T, typename A>
+__global__ __launch_bounds__(64) void attn_forward_row_kernel(AttnParams p) {
+    __shared__ A sp[kWave];
+    const int lane = threadIdx.x;
+    const int64_t row = blockIdx.x;  // (b * H + h) * Q + i
+    const int i = static_cast<int>(row % p.Q), h = static_cast<int>((row / p.Q) % p.H);
+    const int b = static_cast<int>(row / p.Q / p.H), hk = h / p.G;
+    const T* q = at<T>(p.q, p.qs, b, i, h);
+    A m = neg_inf<A>(), l = 0, acc[kMaxPerLane] = {};
+    for (int j0 = 0; j0 < p.K; j0 += kWave) {
+        const int j = j0 + lane;
+        A t = neg_inf<A>(), add;
+        if (j < p.K && !pair_masked<T, A>(p, b, h, i, j, add)) {
+            const T* k = at<T>(p.k, p.ks, b, j, hk);
+            A s = 0;
+            for (int d = 0; d < p.D; ++d) s += cvt<A>(q[d]) * cvt<A>(k[d]);
+            t = s * static_cast<A>(p.scale) + add;
+        }
+        const A m_new = wave_max(m > t ? m : t == t ? t : m);
+        const A from = m_new == neg_inf<A>() ? static_cast<A>(0) : m_new;
+        const A shrink = exp(m - from), e = exp(t - from);
+        m = m_new;
+        l = l * shrink + wave_sum(e);
+        __syncthreads();
+        sp[lane] = e;
+        __syncthreads();
+        const int n = p.K - j0 < kWave ? p.K - j0 : kWave;
+#pragma unroll
+        for (int u = 0; u < kMaxPerLane; ++u) {
+            const int d = u * kWave + lane;
+            if (d >= p.D) break;
+            A o = acc[u] * shrink;
+            for (int x = 0; x < n; ++x)
+                if (sp[x] != 0) o += sp[x] * cvt<A>(at<T>(p.v, p.vs, b, j0 + x, hk)[d]);
+            acc[u] = o;
+        }
+    }
+    T* out = static_cast<T*>(p.out) + ((static_cast<int64_t>(b) * p.Q + i) * p.H + h) * p.D;
+#pragma unroll
+    for (int u = 0; u < kMaxPerLane; ++u) {
+        const int d = u * kWave + lane;
+        if (d < p.D) out[d] = static_cast<T>(l == 0 ? static_cast<A>(0) : acc[u] / l);
+    }
+    if (p.stats != nullptr && lane == 0) {
+        A* st = static_cast<A*>(p.stats) + 2 * row;
+        st[0] = l == 0 ? static_cast<A>(0) : m;
+        st[1] = l == 0 ? static_cast<A>(0) : log(l);
+    }
+}
+
+// delta[row] = grad_out . out of each (b, h, i), one wavefront each
+template <typename T, typename A>
+__global__ __launch_bounds__(64) void attn_delta_row_kernel(AttnParams p) {
+    const int lane = threadIdx.x;
+    const int64_t row = blockIdx.x;
+    const int i = static_cast<int>(row % p.Q), h = static_cast<int>((row / p.Q) % p.H);
+    const int64_t at0 = (((row / p.Q / p.H) * p.Q + i) * p.H + h) * p.D;
+    A s = 0;
+    for (int d = lane; d < p.D; d += kWave)
+        s += cvt<A>(static_cast<const T*>(p.go)[at0 + d]) * cvt<A>(static_cast<const T*>(p.out)[at0 + d]);
+    s = wave_sum(s);
+    if (lane == 0) static_cast<A*>(p.delta)[row] = s;
+}
+
+// The probability of a pair and the gradient of its score: P = exp(t - m - ln l), dS = P (grad_out . v - delta)
+template <typename T, typename A>
+__device__ __forceinline__ void pair_grad(const AttnParams& p, int b, int h, int i, int j, A& prob, A& ds) {
+    A add;
+    prob = ds = 0;
+    if (pair_masked<T, A>(p, b, h, i, j, add)) return;
+    const T* q = at<T>(p.q, p.qs, b, i, h);
+    const T* k = at<T>(p.k, p.ks, b, j, h / p.G);
+    const T* v = at<T>(p.v, p.vs, b, j, h / p.G);
+    const T* g = static_cast<const T*>(p.go) + ((static_cast<int64_t>(b) * p.Q + i) * p.H + h) * p.D;
+    const int64_t row = (static_cast<int64_t>(b) * p.H + h) * p.Q + i;
+    const A* st = static_cast<const A*>(p.stats) + 2 * row;
+    A s = 0, dp = 0;
+    for (int d = 0; d < p.D; ++d) {
+        s += cvt<A>(q[d]) * cvt<A>(k[d]);
+        dp += cvt<A>(g[d]) * cvt<A>(v[d]);
+    }
+    prob = exp(s * static_cast<A>(p.scale) + add - st[0] - st[1]);
+    ds = prob * (dp - static_cast<const A*>(p.delta)[row]);
+}
+
+template <typename T, typename A>
+__global__ __launch_bounds__(64) void attn_dq_row_kernel(AttnParams p) {
+    __shared__ A sd[kWave];
+    const int lane = threadIdx.x;
+    const int64_t row = blockIdx.x;
+    const int i = static_cast<int>(row % p.Q), h = static_cast<int>((row / p.Q) % p.H);
+    const int b = static_cast<int>(row / p.Q / p.H), hk = h / p.G;
+    A acc[kMaxPerLane] = {};
+    for (int j0 = 0; j0 < p.K; j0 += kWave) {
+        A prob = 0, ds = 0;
+        if (j0 + lane < p.K) pair_grad<T, A>(p, b, h, i, j0 + lane, prob, ds);
+        __syncthreads();
+        sd[lane] = ds;
+        __syncthreads();
+        const int n = p.K - j0 < kWave ? p.K - j0 : kWave;
+#pragma unroll
+        for (int u = 0; u < kMaxPerLane; ++u) {
+            const int d = u * kWave + lane;
+            if (d >= p.D) break;
+            for (int x = 0; x < n; ++x)
+                if (sd[x] != 0) acc[u] += sd[x] * cvt<A>(at<T>(p.k, p.ks, b, j0 + x, hk)[d]);
+        }
+    }
+    T* dq = static_cast<T*>(p.dq) + ((static_cast<int64_t>(b) * p.Q + i) * p.H + h) * p.D;
+#pragma unroll
+    for (int u = 0; u < kMaxPerLane; ++u)
+        if (u * kWave + lane < p.D) dq[u * kWave + lane] = static_cast<T>(acc[u] * static_cast<A>(p.scale));
+}
+
+// One wavefront per (b, key head, j): the rows of every head that shares the key, 64 at a time
+template <typename T, typename A>
+__global__ __launch_bounds__(64) void attn_dkv_row_kernel(AttnParams p) {
+    __shared__ A sp[kWave], sd[kWave];
+    const int lane = threadIdx.x;
+    const int64_t id = blockIdx.x;  // (b * Hk + hk) * K + j
+    const int j = static_cast<int>(id % p.K), hk = static_cast<int>((id / p.K) % p.Hk);
+    const int b = static_cast<int>(id / p.K / p.Hk);
+    A dk[kMaxPerLane] = {}, dv[kMaxPerLane] = {};
+    for (int r0 = 0; r0 < p.rows; r0 += kWave) {
+        A prob = 0, ds = 0;
+        const int r = r0 + lane;
+        if (r < p.rows) pair_grad<T, A>(p, b, hk * p.G + r % p.G, r / p.G, j, prob, ds);
+        __syncthreads();
+        sp[lane] = prob;
+        sd[lane] = ds;
+        __syncthreads();
+        const int n = p.rows - r0 < kWave ? p.rows - r0 : kWave;
+#pragma unroll
+        for (int u = 0; u < kMaxPerLane; ++u) {
+            const int d = u * kWave + lane;
+            if (d >= p.D) break;
+            for (int x = 0; x < n; ++x) {
+                const int i = (r0 + x) / p.G, h = hk * p.G + (r0 + x) % p.G;
+                if (sp[x] != 0)
+                    dv[u] += sp[x] * cvt<A>(static_cast<const T*>(
+                                         p.go)[((static_cast<int64_t>(b) * p.Q + i) * p.H + h) * p.D + d]);
+                if (sd[x] != 0) dk[u] += sd[x] * cvt<A>(at<T>(p.q, p.qs, b, i, h)[d]);
+            }
+        }
+    }
+    const int64_t o = ((static_cast<int64_t>(b) * p.K + j) * p.Hk + hk) * p.D;
+#pragma unroll
+    for (int u = 0; u < kMaxPerLane; ++u) {
+        const int d = u * kWave + lane;
+        if (d >= p.D) break;
+        static_cast<T*>(p.dk)[o + d] = static_cast<T>(dk[u] * static_cast<A>(p.scale));
+        static_cast<T*>(p.dv)[o + d] = static_cast<T>(dv[u]);
+    }
+}
+
+int launched(const char* what) {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? 0 : set_error(TD_E_LAUNCH, "%s launch failed: %s", what, hipGetErrorString(e));
+}
+
+template <typename T, typename A>
+int forward_row(const AttnParams& p, hipStream_t stream) {
+    hipLaunchKernelGGL((attn_forward_row_kernel<T, A>), dim3(static_cast<unsigned>(p.B) * p.H * p.Q), dim3(64), 0,
+                       stream, p);
+    return launched("attention");
+}
+
+template <typename T, typename A>
+int backward_row(const AttnParams& p, hipStream_t stream) {
+    const unsigned rows = static_cast<unsigned>(p.B) * p.H * p.Q, keys = static_cast<unsigned>(p.B) * p.Hk * p.K;
+    if (rows > 0) hipLaunchKernelGGL((attn_delta_row_kernel<T, A>), dim3(rows), dim3(64), 0, stream, p);
+    if (rows > 0 && p.dq != nullptr)
+        hipLaunchKernelGGL((attn_dq_row_kernel<T, A>), dim3(rows), dim3(64), 0, stream, p);
+    if (keys > 0 && p.dk != nullptr)
+        hipLaunchKernelGGL((attn_dkv_row_kernel<T, A>), dim3(keys), dim3(64), 0, stream, p);
+    return launched("attention backward");
+}
+
+}  // namespace
+
+int launch_attn_forward_generic(int dtype, const AttnParams& p, hipStream_t stream) {
+    switch (dtype) {
+        case kF32: return forward_row<float, float>(p, stream);
+        case kF16: return forward_row<f16, float>(p, stream);
+        case kBF16: return forward_row<bf16, float>(p, stream);
+        default: return forward_row<double, double>(p, stream);
+    }
+}
+
+int launch_attn_backward_generic(int dtype, const AttnParams& p, hipStream_t stream) {
+    switch (dtype) {
+        case kF32: return backward_row<float, float>(p, stream);
+        case kF16: return backward_row<f16, float>(p, stream);
+        case kBF16: return backward_row<bf16, float>(p, stream);
+        default: return backward_row<double, double>(p, stream);
+    }
+}
+
+AttnParams attn_params(const td_attn_args& a) {
+    AttnParams p{};
+    p.q = a.query;
+    p.k = a.key;
+    p.v = a.value;
+    p.mask = a.mask;
+    p.pad = a.key_padding;
+    p.out = a.out;
+    p.stats = a.stats;
+    for (int i = 0; i < 3; ++i) {
+        p.qs[i] = a.query_stride[i];
+        p.ks[i] = a.key_stride[i];
+        p.vs[i] = a.value_stride[i];
+        p.ms[i] = a.mask_stride[i];
+    }
+    p.B = static_cast<int>(a.B);
+    p.Q = static_cast<int>(a.Q);
+    p.K = static_cast<int>(a.K);
+    p.H = static_cast<int>(a.H);
+    p.Hk = static_cast<int>(a.Hk);
+    p.D = static_cast<int>(a.D);
+    p.G = p.H / p.Hk;
+    p.rows = p.Q * p.G;
+    p.gdiv = make_fastdiv(static_cast<uint32_t>(p.G));
+    p.mask_type = a.mask_type;
+    p.causal = a.causal != 0;
+    p.diag = a.K - a.Q;
+    p.scale = a.scale;
+    p.c = static_cast<float>(a.scale * 1.4426950408889634);
+    return p;
+}
+
+namespace {
+
+constexpr int64_t kIntMax = 2147483647;
+
+int check_args(const td_attn_args* a) {
+    set_error(TD_OK, "");
+    if (a == nullptr) return set_error(TD_E_ARG, "null pointer argument");
+    if (a->dtype < TD_F32 || a->dtype > TD_F64) return set_error(TD_E_DTYPE, "unknown dtype code %d", a->dtype);
+    if (a->B < 0 || a->Q < 0 || a->K < 0) return set_error(TD_E_ARG, "sizes must be non-negative");
+    if (a->H <= 0 || a->Hk <= 0) return set_error(TD_E_ARG, "need at least one head");
+    if (a->H > kIntMax || a->H % a->Hk != 0)
+        return set_error(TD_E_ARG, "the heads of key and value must divide the heads of query");
+    if (a->D < 1 || a->D > TD_ATTN_MAX_HEAD_DIM)
+        return set_error(TD_E_ARG, "head dim must be from 1 to %d", TD_ATTN_MAX_HEAD_DIM);
+    if (a->B > kIntMax || a->Q > kIntMax || a->K > kIntMax || a->H > kIntMax ||
+        static_cast<__int128>(a->B) * a->Q * a->H > kIntMax || static_cast<__int128>(a->B) * a->K * a->Hk > kIntMax)
+        return set_error(TD_E_ARG, "too many (batch, token, head) rows");
+    if (!(a->scale > 0) || !isfinite(a->scale)) return set_error(TD_E_ARG, "scale must be positive and finite");
+    if (a->mask_type < TD_MASK_NONE || a->mask_type > TD_MASK_FLOAT)
+        return set_error(TD_E_ARG, "unknown mask type %d", a->mask_type);
+    return TD_OK;
+}
+
+bool has_queries(const td_attn_args* a) { return a->B * a->Q > 0; }
+bool has_keys(const td_attn_args* a) { return a->B * a->K > 0; }
+
+int check_pointers(const td_attn_args* a) {
+    if (has_queries(a) && (a->query == nullptr || a->out == nullptr))
+        return set_error(TD_E_ARG, "null pointer argument");
+    if (has_keys(a) && (a->key == nullptr || a->value == nullptr)) return set_error(TD_E_ARG, "null pointer argument");
+    if (has_queries(a) && has_keys(a) && a->mask_type != TD_MASK_NONE && a->mask == nullptr)
+        return set_error(TD_E_ARG, "null pointer argument");
+    return TD_OK;
+}
+
+}  // namespace
+}  // namespace td
+
+using namespace td;
+
+extern "C" int64_t td_attn_forward_workspace(const td_attn_args* args) {
+    const int rc = check_args(args);
+    return rc != TD_OK ? rc : 0;
+}
+
+extern "C" int td_attn_forward(const td_attn_args* args, void* workspace, int64_t workspace_bytes, void* stream) {
+    int rc = check_args(args);
+    if (rc == TD_OK) rc = check_pointers(args);
+    if (rc != TD_OK) return rc;
+    if (!has_queries(args)) return TD_OK;
+    return launch_attn_forward_generic(args->dtype, attn_params(*args), static_cast<hipStream_t>(stream));
+}
+
+extern "C" int64_t td_attn_backward_workspace(const td_attn_args* args) {
+    const int rc = check_args(args);
+    return rc != TD_OK ? rc : args->B * args->H * args->Q * (args->dtype == TD_F64 ? 8 : 4);
+}
+
+extern "C" int td_attn_backward(const td_attn_args* args, const void* grad_out, void* grad_query, void* grad_key,
+                                void* grad_value, void* workspace, int64_t workspace_bytes, void* stream) {
+    const int64_t need = td_attn_backward_workspace(args);
+    if (need < 0) return static_cast<int>(need);
+    const int rc = check_pointers(args);
+    if (rc != TD_OK) return rc;
+    if ((has_queries(args) && (grad_out == nullptr || args->stats == nullptr)) ||
+        (grad_key == nullptr) != (grad_value == nullptr))
+        return set_error(TD_E_ARG, "null pointer argument");
+    if (workspace_bytes < need || (need > 0 && workspace == nullptr))
+        return set_error(TD_E_WORKSPACE, "attention backward: the workspace has %lld bytes, %lld are needed",
+                         static_cast<long long>(workspace_bytes), static_cast<long long>(need));
+    if (!has_queries(args) && !has_keys(args)) return TD_OK;
+    AttnParams p = attn_params(*args);
+    p.go = grad_out;
+    p.dq = grad_query;
+    p.dk = grad_key;
+    p.dv = grad_value;
+    p.delta = workspace;
+    return launch_attn_backward_generic(args->dtype, p, static_cast<hipStream_t>(stream));
+}

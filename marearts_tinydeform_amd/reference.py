@@ -92,3 +92,51 @@ def ma_deform_attn_layer_reference(hidden_states, encoder_hidden_states, referen
     if output_weight is not None:
         out = F.linear(out, output_weight, output_bias)
     return (out, attention) if return_attention_weights else out
+
+
+def ma_attn_reference(query, key, value, attn_mask=None, key_padding_mask=None, scale=None, causal=False):
+    """Attention among tokens in PyTorch (ma_attn's arguments and result), computed in float32 (float64 for float64
+    inputs) and rounded once. A query that the masks leave no key gives 0."""
+    B, Q, H, D = query.shape
+    K, G = key.shape[1], H // key.shape[2]
+    acc = torch.float64 if query.dtype == torch.float64 else torch.float32
+    pad = None if key_padding_mask is None else key_padding_mask.bool()[:, :, None, None]
+    if pad is not None:  # an excluded key counts for nothing, whatever it holds
+        key, value = key.masked_fill(pad, 0), value.masked_fill(pad, 0)
+    q = query.to(acc).transpose(1, 2)
+    k, v = (t.to(acc).transpose(1, 2).repeat_interleave(G, 1) for t in (key, value))
+    t = q @ k.transpose(2, 3) * (D ** -0.5 if scale is None else scale)
+    left_out = torch.zeros((), dtype=torch.bool, device=t.device)
+    if attn_mask is not None:
+        if attn_mask.is_floating_point():
+            t = t + attn_mask.to(acc)
+            left_out = left_out | (attn_mask == float('-inf'))
+        else:
+            left_out = left_out | attn_mask.bool()
+    if pad is not None:
+        left_out = left_out | pad.permute(0, 2, 3, 1)
+    if causal:
+        i = torch.arange(Q, device=t.device)[:, None] + (K - Q)
+        left_out = left_out | (torch.arange(K, device=t.device)[None, :] > i)
+    t = t.masked_fill(left_out, float('-inf'))
+    if K > 0:
+        top = t.detach().amax(-1, keepdim=True)
+        t = t - top.masked_fill(top == float('-inf'), 0)
+    e = t.exp()
+    total = e.sum(-1, keepdim=True)
+    out = (e / total.masked_fill(total == 0, 1)) @ v
+    return out.transpose(1, 2).reshape(B, Q, H * D).to(query.dtype)
+
+
+def ma_layer_norm_reference(x, weight=None, bias=None, residual=None, eps=1e-5):
+    """Layer norm of x (+ residual) over the last dimension in PyTorch (ma_layer_norm's arguments and result), computed
+    in float32 (float64 for float64 inputs) and rounded once."""
+    acc = torch.float64 if x.dtype == torch.float64 else torch.float32
+    h = x.to(acc) if residual is None else x.to(acc) + residual.to(acc)
+    h = h - h.mean(-1, keepdim=True)
+    h = h * torch.rsqrt((h * h).mean(-1, keepdim=True) + eps)
+    if weight is not None:
+        h = h * weight.to(acc)
+    if bias is not None:
+        h = h + bias.to(acc)
+    return h.to(x.dtype)

@@ -1,0 +1,270 @@
+"""Attention among tokens on the GPU against the float64 oracle (oracle/dense.py), within the bounds that its
+attn_bounds derives: forward, backward, every mask, strides, streams, graphs and the C ABI's buffers."""
+
+import numpy as np
+import pytest
+import torch
+
+import marearts_tinydeform_amd as td
+from marearts_tinydeform_amd import _dense, _native
+from oracle import dense
+from dense_cases import ATTN_SIZES, MASKS, agree, check_attn, half_steps, make_attn
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def say(msg):
+    print(msg, flush=True)
+
+
+def on_gpu(kw):
+    return {n: t.cuda() if isinstance(t, torch.Tensor) else t for n, t in kw.items()}
+
+
+def run(q, k, v, go, kw, train=True):
+    """(out, grads) of the GPU entries for CPU inputs"""
+    kw = on_gpu(kw)
+    a, b, c = (t.cuda().requires_grad_(train) for t in (q, k, v))
+    if not train:
+        with torch.inference_mode():
+            out = td.ma_attn(a, b, c, **kw)
+        torch.cuda.synchronize()
+        return out, None
+    out = td.ma_attn_train(a, b, c, **kw)
+    grads = torch.autograd.grad(out, (a, b, c), go.cuda())
+    torch.cuda.synchronize()
+    return out, grads
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('size', ATTN_SIZES, ids=str)
+def test_sizes(size, dtype):
+    say(f'  attention {size} {dtype}')
+    q, k, v, go, kw = make_attn(size, dtype)
+    out, grads = run(q, k, v, go, kw)
+    check_attn(dtype, q, k, v, go, kw, out, grads)
+    again, _ = run(q, k, v, go, kw, train=False)
+    assert torch.equal(again, out), 'inference and training forward differ'
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('mask', MASKS[1:])
+def test_masks(mask, dtype):
+    for i, size in enumerate([(2, 45, 100, 2, 2, 32), (1, 130, 70, 4, 2, 64), (3, 5, 300, 4, 1, 36),
+                              (2, 150, 150, 2, 2, 32), (2, 1, 513, 4, 4, 128)]):
+        say(f'  attention {mask} {size} {dtype}')
+        q, k, v, go, kw = make_attn(size, dtype, mask, seed=i)
+        out, grads = run(q, k, v, go, kw)
+        check_attn(dtype, q, k, v, go, kw, out, grads)
+        again, _ = run(q, k, v, go, kw, train=False)
+        assert torch.equal(again, out), 'inference and training forward differ'
+
+
+@pytest.mark.parametrize('mask', ['none', 'bool', 'float', 'lowest', 'all'])
+def test_float64(mask):
+    for size in [(2, 33, 70, 4, 2, 36), (1, 1, 65, 2, 2, 128)]:
+        q, k, v, go, kw = make_attn(size, torch.float64, mask)
+        out, grads = run(q, k, v, go, kw)
+        check_attn(torch.float64, q, k, v, go, kw, out, grads)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_a_row_left_nothing_gives_zeros(dtype):
+    q, k, v, go, _ = make_attn((2, 40, 50, 2, 2, 32), dtype)
+    mask = torch.zeros(2, 1, 40, 50, dtype=torch.bool)
+    mask[0, 0, 3] = True
+    mask[1] = True
+    out, (dq, dk, dv) = run(q, k, v, go, dict(attn_mask=mask))
+    out = out.detach()
+    assert float(out[0, 3].abs().sum()) == 0 and float(out[1].abs().sum()) == 0
+    assert float(dq[0, 3].abs().sum()) == 0 and float(dq[1].abs().sum()) == 0
+    assert float(dk[1].abs().sum()) == 0 and float(dv[1].abs().sum()) == 0
+    assert float(out[0].abs().sum()) > 0 and torch.isfinite(dk).all()
+
+
+@pytest.mark.parametrize('dtype', TYPES + [torch.float64])
+def test_padded_keys_count_for_nothing_whatever_they_hold(dtype):
+    q, k, v, go, _ = make_attn((2, 40, 90, 2, 2, 32), dtype)
+    pad = torch.zeros(2, 90, dtype=torch.bool)
+    pad[0, 70:] = True
+    pad[1, ::3] = True
+    clean = run(q, k, v, go, dict(key_padding_mask=pad))
+    for value in (float('nan'), float('inf'), -float('inf')):
+        k2, v2 = k.clone(), v.clone()
+        k2[pad], v2[pad] = value, value
+        out, grads = run(q, k2, v2, go, dict(key_padding_mask=pad))
+        assert torch.equal(out, clean[0])
+        for a, b in zip(grads, clean[1]):
+            assert torch.equal(a, b)
+        assert float(grads[1][pad.cuda()].abs().sum()) == 0 and float(grads[2][pad.cuda()].abs().sum()) == 0
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_large_scores(dtype):
+    # scores of hundreds: one key takes nearly all of each row, the others underflow
+    q, k, v, go, _ = make_attn((1, 60, 130, 2, 2, 32), dtype)
+    q, k = q * 8, k * 8
+    out, grads = run(q, k, v, go, {})
+    check_attn(dtype, q, k, v, go, {}, out, grads)
+    # the first keys' scores far below the last ones': the running maximum moves on every tile
+    k = (k.float() * torch.linspace(0.01, 2, 130)[None, :, None, None]).to(dtype)
+    out, grads = run(q, k, v, go, {})
+    check_attn(dtype, q, k, v, go, {}, out, grads)
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
+def test_small_and_large_gradients(dtype):
+    # gradients of a loss over many tokens (1e-4) and of a scaled loss (1e3): dS is rounded to 16 bits
+    for scale in (1e-4, 1e3):
+        q, k, v, go, kw = make_attn((1, 100, 700, 2, 2, 32), dtype, grad_scale=scale)
+        out, grads = run(q, k, v, go, kw)
+        check_attn(dtype, q, k, v, go, kw, out, grads)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_strides(dtype):
+    B, N, H, D = 2, 70, 3, 32
+    q, k, v, go, _ = make_attn((B, N, N, H, H, D), dtype)
+    want, wgrads = run(q, k, v, go, {})
+    joint = torch.stack([q, k, v], 2).cuda()                            # slices of a joint projection
+    heads = [t.transpose(1, 2).contiguous().transpose(1, 2).cuda() for t in (q, k, v)]   # head-major
+    odd = torch.zeros(B * N * H * D + 1, dtype=dtype, device='cuda')     # off 16-byte boundaries
+    odd = [torch.cat([odd[:1], t.cuda().flatten()])[1:].view(B, N, H, D) for t in (q, k, v)]
+    wide = [torch.cat([t, t[..., :5]], -1).cuda()[..., :D] for t in (q, k, v)]           # head rows of 37 elements
+    last = [t.transpose(1, 3).contiguous().transpose(1, 3).cuda() for t in (q, k, v)]    # last dimension strided
+    for name, ts in (('joint', joint.unbind(2)), ('heads', heads), ('odd', odd), ('wide', wide), ('last', last)):
+        say(f'  strides {name} {dtype}')
+        ts = [t.detach().requires_grad_() for t in ts]
+        out = td.ma_attn_train(*ts)
+        grads = torch.autograd.grad(out, ts, go.cuda())
+        check_attn(dtype, q, k, v, go, {}, out, grads)
+    one = k[:1].cuda().requires_grad_()                                 # one image's keys for the whole batch
+    val = v[:1].cuda().requires_grad_()
+    qg = q.cuda().requires_grad_()
+    out = td.ma_attn_train(qg, one.expand(B, N, H, D), val.expand(B, N, H, D))
+    grads = torch.autograd.grad(out, (qg, one, val), go.cuda())
+    k2, v2 = k[:1].expand(B, N, H, D), v[:1].expand(B, N, H, D)
+    r = dense.attn(q, k2, v2, grad_out=go)
+    u = half_steps(dtype)[0]
+    b = dense.attn_bounds(r, *half_steps(dtype))
+    agree(out, r['out'], b['out'], 1e-6, 'broadcast out')
+    for name, t in (('dk', grads[1]), ('dv', grads[2])):                # autograd adds the images' in dtype: 2 u more
+        ref = r[name].sum(0, keepdims=True)
+        agree(t, ref, b[name].sum(0, keepdims=True) + 2 * u * np.abs(r[name]).sum(0, keepdims=True), 1e-6, name)
+    # a mask with strides of its own, and a non-contiguous incoming gradient
+    big = torch.rand(N, 2 * N, generator=torch.Generator().manual_seed(1)) < 0.5
+    m, gt = big[:, ::2], go.transpose(0, 1).contiguous().transpose(0, 1)
+    for mm in (m, big[:, :N], m.t().contiguous().t()):
+        ts = [t.cuda().requires_grad_() for t in (q, k, v)]
+        out = td.ma_attn_train(*ts, attn_mask=mm.cuda())
+        grads = torch.autograd.grad(out, ts, gt.cuda())
+        check_attn(dtype, q, k, v, go, dict(attn_mask=mm.contiguous()), out, grads)
+
+
+def test_some_gradients_only():
+    q, k, v, go, _ = make_attn((1, 30, 40, 2, 2, 32), torch.float32)
+    _, want = run(q, k, v, go, {})
+    for pick in ((0,), (1,), (2,), (0, 2)):
+        ts = [t.cuda().requires_grad_(i in pick) for i, t in enumerate((q, k, v))]
+        grads = torch.autograd.grad(td.ma_attn_train(*ts), [ts[i] for i in pick], go.cuda())
+        for i, g in zip(pick, grads):
+            assert torch.equal(g, want[i])
+
+
+def test_nothing_to_attend_to():
+    for B, Q, K in ((0, 3, 4), (2, 0, 4), (2, 3, 0), (2, 0, 0)):
+        ts = [torch.randn(B, n, 2, 8, device='cuda').requires_grad_() for n in (Q, K, K)]
+        out = td.ma_attn_train(*ts)
+        assert out.shape == (B, Q, 16) and float(out.detach().abs().sum()) == 0
+        for t, g in zip(ts, torch.autograd.grad(out, ts, torch.ones_like(out))):
+            assert g.shape == t.shape and float(g.abs().sum()) == 0
+
+
+def test_refuses_gradients_in_the_inference_entry():
+    t = torch.randn(1, 4, 2, 8, device='cuda', requires_grad=True)
+    with pytest.raises(RuntimeError, match='inference only'):
+        td.ma_attn(t, t, t)
+    with pytest.raises(RuntimeError, match='attn_mask has no gradient'):
+        td.ma_attn_train(t, t, t, attn_mask=torch.zeros(4, 4, device='cuda', requires_grad=True))
+    out = td.ma_attn_train(t, t, t)
+    g, = torch.autograd.grad(out, t, torch.ones_like(out).requires_grad_(), create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), t)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_the_same_on_every_run_and_on_another_stream(dtype):
+    q, k, v, go, kw = make_attn((2, 200, 333, 4, 2, 64), dtype, 'padding')
+    want = run(q, k, v, go, kw)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = run(q, k, v, go, kw)
+    torch.cuda.current_stream().wait_stream(s)
+    for a, b in zip((want[0],) + want[1], (got[0],) + got[1]):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.float32])
+def test_graphs_replay_forward_and_backward(dtype):
+    """Two captured graphs (a training step each, other sizes) and eager work in between: every replay is the eager
+    result. The leaves of a captured step have no eager graph alive, as torch asks of captured backward passes."""
+    graphs = []
+    for size, mask in (((2, 100, 100, 4, 4, 32), 'bool'), ((1, 2, 3000, 8, 2, 64), 'padding')):
+        q, k, v, go, kw = make_attn(size, dtype, mask)
+        want, wgrads = run(q, k, v, go, kw)
+        ts = [t.cuda().requires_grad_() for t in (q, k, v)]
+        kw, g = on_gpu(kw), go.cuda()
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            torch.autograd.grad(td.ma_attn_train(*ts, **kw), ts, g)
+        torch.cuda.current_stream().wait_stream(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = td.ma_attn_train(*ts, **kw)
+            grads = torch.autograd.grad(out, ts, g)
+        graphs.append((graph, (out.detach(),) + grads, (want,) + wgrads, (ts, kw, g)))
+    for i in range(3):
+        for graph, got, want, _ in graphs:
+            for t in got:
+                t.zero_()
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, got, want, (ts, kw, g) in graphs:
+            for a, b in zip(got, want):
+                assert torch.equal(a, b), f'replay {i}'
+            with torch.inference_mode():
+                assert torch.equal(td.ma_attn(*[t.detach() for t in ts], **kw), want[0])
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_c_abi_writes_its_buffers_and_nothing_else(dtype):
+    for size in [(1, 33, 70, 4, 2, 36), (2, 1, 2000, 4, 1, 64), (1, 130, 60, 2, 2, 32)]:
+        B, Q, K, H, Hk, D = size
+        q, k, v, go, _ = make_attn(size, dtype)
+        q, k, v, go = (t.cuda() for t in (q, k, v, go))
+        lib, acc = _native.lib, torch.float32
+        fence = 64
+
+        def fenced(n, dt):
+            t = torch.full((n + 2 * fence,), 7.0, dtype=dt, device='cuda')
+            return t, t[fence:fence + n]
+        bufs = [fenced(B * Q * H * D, dtype), fenced(B * H * Q * 2, acc), fenced(B * Q * H * D, dtype),
+                fenced(B * K * Hk * D, dtype), fenced(B * K * Hk * D, dtype)]
+        out, stats, dq, dk, dv = (b[1] for b in bufs)
+        args = _dense._pack(q, k, v, None, 0, (0, 0, 0), None, D ** -0.5, False, out, stats)
+        need = lib.td_attn_forward_workspace(args)
+        w1 = fenced(max(need, 4) // 4, torch.float32)
+        assert lib.td_attn_forward(args, w1[1].data_ptr(), need, None) == 0
+        need = lib.td_attn_backward_workspace(args)
+        w2 = fenced(max(need, 4) // 4, torch.float32)
+        assert lib.td_attn_backward(args, go.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), w2[1].data_ptr(),
+                                    need, None) == 0
+        torch.cuda.synchronize()
+        for whole, part in bufs + [w1, w2]:
+            n = part.numel()
+            assert (whole[:fence] == 7).all() and (whole[fence + n:] == 7).all()
+        check_attn(dtype, q.cpu(), k.cpu(), v.cpu(), go.cpu(), {}, out.view(B, Q, H * D),
+                   (dq.view(q.shape), dk.view(k.shape), dv.view(v.shape)))
