@@ -28,7 +28,10 @@ ARCH = 'gfx950'
 
 SOURCES = ['td_abi.hip', 'td_fused.hip', 'td_sample.hip', 'td_gemm.hip', 'td_gemm_dma.hip', 'td_gemm_stream.hip',
            'td_gemm_split.hip', 'td_layer.hip', 'td_backward.hip', 'td_noalloc.hip', 'td_probe.hip', 'td_attn.hip',
-           'td_norm.hip']
+           'td_attn_forward.hip', 'td_norm.hip']
+
+# compiled once per element type (TD_ATTN_TYPE 0 float32, 1 float16, 2 bfloat16), so that the types build in parallel
+BY_TYPE = ['td_attn_forward.hip']
 
 # per-source additions: the direct-to-LDS GEMM keeps its MFMA accumulators in architectural VGPRs (in the
 # accumulator-register form the compiler copies every accumulator through a temporary in the inner loop)
@@ -51,9 +54,12 @@ def hipcc():
 
 
 def _compile(job):
-    src, phases = job
-    obj = os.path.join(BUILD, os.path.splitext(src)[0] + ('_phases' if phases else '') + '.o')
+    src, phases, kind = job
+    obj = os.path.join(BUILD, os.path.splitext(src)[0] + ('_phases' if phases else '')
+                       + ('' if kind is None else f'_{kind}') + '.o')
     defs = ['-DTD_PHASE_STAMPS'] if phases else []
+    if kind is not None:
+        defs.append(f'-DTD_ATTN_TYPE={kind}')
     cmd = [hipcc()] + HIPCC_FLAGS + EXTRA_FLAGS.get(src, []) + defs + ['-c', os.path.join(CSRC, src), '-o', obj]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
@@ -74,19 +80,20 @@ def build(verbose=False, phases=True):
     """Compile every HIP source and link libtinydeform.so (and, with phases, libtinydeform_phases.so); returns the
     library path."""
     os.makedirs(BUILD, exist_ok=True)
-    jobs = [(src, False) for src in SOURCES] + ([(PHASES_SOURCE, True)] if phases else [])
-    # the two largest sources first, so that they do not start last
-    jobs.sort(key=lambda j: j[0] != PHASES_SOURCE)
+    jobs = [(src, False, kind) for src in SOURCES for kind in (range(3) if src in BY_TYPE else [None])]
+    jobs += [(PHASES_SOURCE, True, None)] if phases else []
+    # the largest sources first, so that they do not start last
+    jobs.sort(key=lambda j: j[0] not in BY_TYPE + [PHASES_SOURCE])
     workers = min(len(jobs), max(1, (os.cpu_count() or 2) // 2))
     with concurrent.futures.ThreadPoolExecutor(workers) as ex:
         objs = list(ex.map(_compile, jobs))
-    plain = [o for o, (_, ph) in zip(objs, jobs) if not ph]
+    plain = [o for o, (_, ph, _) in zip(objs, jobs) if not ph]
     _link(plain, LIB)
     if verbose:
         print('built', LIB)
     if phases:
         swap = {os.path.join(BUILD, os.path.splitext(PHASES_SOURCE)[0] + '.o'): o
-                for o, (_, ph) in zip(objs, jobs) if ph}
+                for o, (_, ph, _) in zip(objs, jobs) if ph}
         _link([swap.get(o, o) for o in plain], PHASES_LIB)
         if verbose:
             print('built', PHASES_LIB)

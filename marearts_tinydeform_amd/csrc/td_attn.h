@@ -12,7 +12,8 @@ namespace td {
 struct AttnParams {
     const void *q, *k, *v, *mask;
     const uint8_t* pad;
-    void *out, *stats;
+    void *out;
+    void *stats;  // [B, H, Q, 2]: the maximum of each row's scores and log2 of the sum of 2^(score - maximum), in base 2
     int64_t qs[3], ks[3], vs[3], ms[3];  // batch, token (query), head strides in elements
     int B, Q, K, H, Hk, D, G;
     int rows;       // Q * G
@@ -31,6 +32,14 @@ struct AttnParams {
 };
 
 AttnParams attn_params(const td_attn_args& a);
+
+// On the matrix units, for float32, float16 and bfloat16 (td_attn_forward.hip)
+int64_t attn_forward_workspace(int dtype, const AttnParams& p);
+int launch_attn_forward(int dtype, const AttnParams& p, hipStream_t stream);
+template <typename T>
+int launch_attn_forward_t(int dtype, const AttnParams& p, hipStream_t stream);
+// Head widths the matrix-unit kernels are built for
+inline int padded_width(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
 // Every launcher returns 0 or a negative TD_E* code after recording a message.
 int launch_attn_forward_generic(int dtype, const AttnParams& p, hipStream_t stream);

@@ -12,13 +12,16 @@ __device__ __forceinline__ const T* at(const void* base, const int64_t (&s)[3], 
     return static_cast<const T*>(base) + b * s[0] + static_cast<int64_t>(tok) * s[1] + h * s[2];
 }
 
+constexpr double kLog2eD = 1.4426950408889634;
+
 template <typename A>
 constexpr A neg_inf() {
     return -static_cast<A>(__builtin_inf());
 }
 
-// Whether (query i, key j) is left out by causal, padding or the mask, and the additive mask's term. A -inf of a float
-// mask leaves the pair out whatever its score is.
+// Whether (query i, key j) is left out by causal, padding or the mask, and the additive mask's term in base 2 (its lowest
+// value kept finite, so that a row of it alone is a uniform row). A -inf of a float mask leaves the pair out whatever its
+// score is.
 template <typename T, typename A>
 __device__ __forceinline__ bool pair_masked(const AttnParams& p, int b, int h, int i, int j, A& add) {
     add = static_cast<A>(0);
@@ -28,7 +31,17 @@ __device__ __forceinline__ bool pair_masked(const AttnParams& p, int b, int h, i
     const int64_t m = b * p.ms[0] + h * p.ms[1] + i * p.ms[2] + j;
     if (p.mask_type == TD_MASK_BYTES) return static_cast<const uint8_t*>(p.mask)[m] != 0;
     add = cvt<A>(static_cast<const T*>(p.mask)[m]);
-    return add == neg_inf<A>();
+    if (add == neg_inf<A>()) return true;
+    const A lowest = static_cast<A>(sizeof(A) == 8 ? -1.7976931348623157e308 : -3.4028234663852886e38);
+    add *= static_cast<A>(kLog2eD);
+    if (add < lowest) add = lowest;
+    return false;
+}
+
+// scores are in base 2: c = scale * log2(e)
+template <typename A>
+__device__ __forceinline__ A score_factor(const AttnParams& p) {
+    return static_cast<A>(p.scale * kLog2eD);
 }
 
 template <typename A>
@@ -62,11 +75,11 @@ __global__ __launch_bounds__(64) void attn_forward_row_kernel(AttnParams p) {
             const T* k = at<T>(p.k, p.ks, b, j, hk);
             A s = 0;
             for (int d = 0; d < p.D; ++d) s += cvt<A>(q[d]) * cvt<A>(k[d]);
-            t = s * static_cast<A>(p.scale) + add;
+            t = s * score_factor<A>(p) + add;
         }
         const A m_new = wave_max(m > t ? m : t == t ? t : m);
         const A from = m_new == neg_inf<A>() ? static_cast<A>(0) : m_new;
-        const A shrink = exp(m - from), e = exp(t - from);
+        const A shrink = exp2(m - from), e = exp2(t - from);
         m = m_new;
         l = l * shrink + wave_sum(e);
         __syncthreads();
@@ -92,7 +105,7 @@ __global__ __launch_bounds__(64) void attn_forward_row_kernel(AttnParams p) {
     if (p.stats != nullptr && lane == 0) {
         A* st = static_cast<A*>(p.stats) + 2 * row;
         st[0] = l == 0 ? static_cast<A>(0) : m;
-        st[1] = l == 0 ? static_cast<A>(0) : log(l);
+        st[1] = l == 0 ? static_cast<A>(0) : log2(l);
     }
 }
 
@@ -110,7 +123,7 @@ __global__ __launch_bounds__(64) void attn_delta_row_kernel(AttnParams p) {
     if (lane == 0) static_cast<A*>(p.delta)[row] = s;
 }
 
-// The probability of a pair and the gradient of its score: P = exp(t - m - ln l), dS = P (grad_out . v - delta)
+// The probability of a pair and the gradient of its score: P = 2^(t - m - log2 l), dS = P (grad_out . v - delta)
 template <typename T, typename A>
 __device__ __forceinline__ void pair_grad(const AttnParams& p, int b, int h, int i, int j, A& prob, A& ds) {
     A add;
@@ -127,7 +140,7 @@ __device__ __forceinline__ void pair_grad(const AttnParams& p, int b, int h, int
         s += cvt<A>(q[d]) * cvt<A>(k[d]);
         dp += cvt<A>(g[d]) * cvt<A>(v[d]);
     }
-    prob = exp(s * static_cast<A>(p.scale) + add - st[0] - st[1]);
+    prob = exp2(s * score_factor<A>(p) + add - st[0] - st[1]);
     ds = prob * (dp - static_cast<const A*>(p.delta)[row]);
 }
 
@@ -318,7 +331,7 @@ using namespace td;
 
 extern "C" int64_t td_attn_forward_workspace(const td_attn_args* args) {
     const int rc = check_args(args);
-    return rc != TD_OK ? rc : 0;
+    return rc != TD_OK ? rc : args->B * args->Q == 0 ? 0 : attn_forward_workspace(args->dtype, attn_params(*args));
 }
 
 extern "C" int td_attn_forward(const td_attn_args* args, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -326,7 +339,14 @@ extern "C" int td_attn_forward(const td_attn_args* args, void* workspace, int64_
     if (rc == TD_OK) rc = check_pointers(args);
     if (rc != TD_OK) return rc;
     if (!has_queries(args)) return TD_OK;
-    return launch_attn_forward_generic(args->dtype, attn_params(*args), static_cast<hipStream_t>(stream));
+    AttnParams p = attn_params(*args);
+    const int64_t need = attn_forward_workspace(args->dtype, p);
+    if (workspace_bytes < need || (need > 0 && workspace == nullptr))
+        return set_error(TD_E_WORKSPACE, "attention: the workspace has %lld bytes, %lld are needed",
+                         static_cast<long long>(workspace_bytes), static_cast<long long>(need));
+    p.ws = workspace;
+    if (args->dtype == TD_F64) return launch_attn_forward_generic(args->dtype, p, static_cast<hipStream_t>(stream));
+    return launch_attn_forward(args->dtype, p, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int64_t td_attn_backward_workspace(const td_attn_args* args) {

@@ -1,0 +1,431 @@
+// Attention among tokens, forward, on the matrix units (float32, float16, bfloat16).
+//
+// One pass over the keys with the running maximum m and sum l of the softmax (Milakov and Gimelshein, "Online normalizer
+// calculation for softmax", 2018): S^T = K Q^T, P^T = 2^(S^T - m), O^T += V^T P^T, all three transposed, so that a
+// lane's scores are of one row (its column), the row's statistics are one number a lane, and P^T is the second product's
+// operand as it stands in the accumulator.
+#include "td_attn_mma.h"
+
+// The build compiles this file once per type: TD_ATTN_TYPE 0 float32 (and the entry), 1 float16, 2 bfloat16.
+#ifndef TD_ATTN_TYPE
+#error "TD_ATTN_TYPE"
+#endif
+
+namespace td {
+namespace {
+
+// Rescaling O and l is put off until a row's maximum has grown by more than this (base 2): the sums then hold factors of
+// up to 2^kSlack, and only tiles that move a maximum pay for the rescale.
+constexpr float kSlack = 4.f;
+// float16 holds P as 2^11 P (at most 2^(11 + kSlack) < 65504): small probabilities keep their bits down to 2^-25 and
+// steps of 2^-35. The factor is in l as well and cancels.
+template <typename T>
+constexpr float kShift = std::is_same<T, f16>::value ? 11.f : 0.f;
+
+struct Split {
+    int n;      // key ranges a row's keys are split over (1: none)
+    int keys;   // keys of a range, a multiple of 64
+    float* o;   // [n][B * H * Q][D] unnormalised outputs
+    float* ml;  // [n][B * H * Q][2] maximum and sum
+};
+
+// Keys of a tile: 64 where the staged rows leave room for two workgroups on a CU
+template <typename T, int DP, bool WK>
+constexpr int key_tile() {
+    return WK || DP * static_cast<int>(sizeof(T)) > 256 ? 32 : 64;
+}
+
+// Wavefronts a SIMD that the registers have to leave room for (without spills)
+template <typename T, int DP, bool WK, bool SLOW>
+constexpr int min_waves() {
+    constexpr int bytes = DP * static_cast<int>(sizeof(T));
+    constexpr int n = bytes <= 64 ? 4 : bytes <= 128 ? 3 : bytes <= 256 ? 2 : 1;
+    return n > 1 && bytes <= 128 && (WK || SLOW) ? n - 1 : SLOW ? 1 : n;
+}
+
+// WK false: four wavefronts of 32 rows each share the key tiles of the workgroup's 128 rows. WK true: the workgroup has
+// 32 rows and each wavefront every fourth key tile, in LDS of its own; the four partial results are joined in LDS.
+// MASK: there is a mask tensor. VEC: operands are read 16 bytes at a time (StagedRows).
+template <typename T, int DP, bool WK, bool MASK, bool VEC>
+__global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forward_kernel(AttnParams p, Split sp, bool vec_out,
+                                                                               int tiles) {
+    using R = TileRows<T, DP>;
+    constexpr int KT = key_tile<T, DP, WK>(), NT = WK ? 64 : 256, ND = DP / 32;
+    constexpr int kTile = KT * R::kPitch;
+    extern __shared__ __align__(16) unsigned char lds[];
+    const int id = xcd_order(static_cast<int>(blockIdx.x), p.B * p.Hk * tiles * sp.n);
+    if (id < 0) return;
+    const int split = id % sp.n, tile = tiles - 1 - id / sp.n % tiles, bh = id / sp.n / tiles;  // causal: long ones first
+    const int b = bh / p.Hk, hk = bh % p.Hk;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    const int lane = threadIdx.x % kWave, half = lane >> 5;
+    const int t = WK ? lane : static_cast<int>(threadIdx.x);
+    unsigned char* const kt_lds = lds + (WK ? wave * 2 * kTile : 0);
+    unsigned char* const vt_lds = kt_lds + kTile;
+
+    // the lane's row
+    const int row0 = tile * (WK ? 32 : 128), wrow0 = row0 + (WK ? 0 : wave * 32), r = wrow0 + (lane & 31);
+    const bool live = r < p.rows;
+    const int i = static_cast<int>(fast_div(p.gdiv, static_cast<uint32_t>(live ? r : 0)));
+    const int h = hk * p.G + (live ? r : 0) - i * p.G;
+    u32x4 qf[R::kChunks];
+    {
+        const T* q = static_cast<const T*>(p.q) + b * p.qs[0] + i * p.qs[1] + h * p.qs[2];
+#pragma unroll
+        for (int c = 0; c < R::kChunks; ++c)
+            qf[c] = live ? row_piece<T, VEC>(q, c * 32 + half * 16, p.D) : u32x4{0u, 0u, 0u, 0u};
+    }
+    const unsigned char* const mrow =
+        !MASK
+            ? nullptr
+            : static_cast<const unsigned char*>(p.mask) + (b * p.ms[0] + h * p.ms[1] + i * p.ms[2]) *
+                                                              (p.mask_type == TD_MASK_FLOAT ? sizeof(T) : 1);
+    const int diag = static_cast<int>(p.diag);
+    const int last = p.causal ? i + diag : 2147483647;
+
+    // the workgroup's keys, and the wavefront's first and last row's
+    int kend = p.K, k0 = 0;
+    const int top_row = (row0 + (WK ? 32 : 128) < p.rows ? row0 + (WK ? 32 : 128) : p.rows) - 1;
+    if (p.causal) {
+        const int seen = static_cast<int>(fast_div(p.gdiv, static_cast<uint32_t>(top_row))) + diag + 1;
+        kend = seen < kend ? seen : kend;
+    }
+    if (sp.n > 1) {
+        k0 = split * sp.keys;
+        kend = k0 + static_cast<int64_t>(sp.keys) < kend ? k0 + sp.keys : kend;
+    }
+    const int wtop = wrow0 + 31 < p.rows ? wrow0 + 31 : p.rows - 1;
+    const int wfirst = wrow0 < p.rows ? wrow0 : p.rows - 1;
+    const int seen_all = p.causal ? static_cast<int>(fast_div(p.gdiv, static_cast<uint32_t>(wfirst))) + diag : 2147483647;
+    const int seen_any = p.causal ? static_cast<int>(fast_div(p.gdiv, static_cast<uint32_t>(wtop))) + diag : 2147483647;
+
+    const T* const kb = static_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[2];
+    const T* const vb = static_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[2];
+    const uint8_t* const pad = p.pad == nullptr ? nullptr : p.pad + static_cast<int64_t>(b) * p.K;
+    // keys j0 + lane of a tile: whether nobody sees them
+    auto pad_byte = [&](int64_t j0) -> int {
+        const int64_t j = j0 + lane;
+        return lane >= KT || j >= kend || (pad != nullptr && pad[j] != 0);
+    };
+
+    StagedRows<T, DP, KT, NT, VEC> ks, vs;
+    auto k_row = [&](int x) { return x * p.ks[1]; };
+    auto v_row = [&](int x) { return x * p.vs[1]; };
+    ks.plan(k_row, p.D, t);
+    vs.plan(v_row, p.D, t);
+    float m = kNegInf, l = 0.f;
+    f32x16 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[d] = f32x16{0.f};
+
+    constexpr int step = WK ? 4 * KT : KT;
+    constexpr uint64_t all = KT == 64 ? ~uint64_t{0} : (uint64_t{1} << (KT & 63)) - 1;
+    int64_t j0 = k0 + (WK ? wave * KT : 0);
+    uint64_t gone = __ballot(pad_byte(j0)), gone_next;
+    auto fetch = [&](int64_t at, uint64_t g) {
+        ks.load(kb + at * p.ks[1], k_row, g & all, p.D, t);
+        vs.load(vb + at * p.vs[1], v_row, g & all, p.D, t);
+    };
+    if (j0 < kend) fetch(j0, gone);
+    int next_pad = pad_byte(j0 + step);
+    for (; j0 < kend; j0 += step) {
+        if (!WK) __syncthreads();
+        ks.store(kt_lds, t);
+        vs.store(vt_lds, t);
+        if (WK)
+            wave_sync();
+        else
+            __syncthreads();
+        gone_next = __ballot(next_pad);
+        if (j0 + step < kend) {
+            fetch(j0 + step, gone_next);
+            next_pad = pad_byte(j0 + 2 * step);
+        }
+        const int j = static_cast<int>(j0);
+        if ((gone & all) != all && j <= seen_any) {
+            const bool whole = j + KT <= p.K;
+            const bool masked = (gone & all) != 0 || mrow != nullptr || j + KT - 1 > seen_all;
+            f32x16 s[KT / 32];
+#pragma unroll
+            for (int x = 0; x < KT / 32; ++x) {
+                s[x] = f32x16{0.f};
+#pragma unroll
+                for (int c = 0; c < R::kChunks; ++c)
+                    s[x] = Mma<T>::mul(R::rows(kt_lds, 32 * x, c, lane), qf[c], s[x]);
+            }
+            float cc = p.c;
+            if (masked) {
+                cc = 1.f;
+#pragma unroll
+                for (int x = 0; x < KT / 32; ++x)
+                    mask_scores<T>(s[x], p, j + 32 * x, static_cast<unsigned>(gone >> (32 * x + 4 * half)), last, mrow,
+                                   half, whole);
+            }
+            float mt = kNegInf;
+#pragma unroll
+            for (int x = 0; x < KT / 32; ++x)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) mt = __builtin_fmaxf(mt, s[x][e]);
+            mt = __builtin_fmaxf(mt, other_half(mt)) * cc;
+            if (__any(mt > m + kSlack)) {
+                const float to = __builtin_fmaxf(m, mt);
+                const float shrink = to == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m - to);
+                m = to;
+                l *= shrink;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) o[d] *= shrink;
+            }
+            const float from = m == kNegInf ? 0.f : m - kShift<T>;
+#pragma unroll
+            for (int x = 0; x < KT / 32; ++x) {
+                f32x16 pr;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    pr[e] = __builtin_amdgcn_exp2f(fmaf(s[x][e], cc, -from));
+                    l += pr[e];
+                }
+                typename R::Packed w[R::kPacked];
+                R::pack(pr, w);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) o[d] = R::columns(vt_lds, 32 * x, 32 * d, lane, w, o[d]);
+            }
+        }
+        gone = gone_next;
+        if (WK) wave_sync();
+    }
+    l += other_half(l);
+
+    if constexpr (WK) {
+        // join the four wavefronts' parts: maxima and sums first, then each scaled O, through LDS
+        __syncthreads();
+        float* const ml = reinterpret_cast<float*>(lds);  // [4][32][2]
+        if (half == 0) {
+            ml[(wave * 32 + lane) * 2] = m;
+            ml[(wave * 32 + lane) * 2 + 1] = l;
+        }
+        __syncthreads();
+        float to = kNegInf, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) to = __builtin_fmaxf(to, ml[(w * 32 + (lane & 31)) * 2]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float mw = ml[(w * 32 + (lane & 31)) * 2], lw = ml[(w * 32 + (lane & 31)) * 2 + 1];
+            sum += mw == kNegInf ? lw : lw * __builtin_amdgcn_exp2f(mw - to);
+        }
+        const float scale = m == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m - to);
+        m = to;
+        l = sum;
+        // [4 waves][32 rows][DP] in two halves of the wavefronts: 2, 3 write and 0, 1 add, then 1 writes and 0 adds
+        float* const part = ml + 256;
+        const int at = (lane & 31) * (DP + 4) + 4 * half;
+        constexpr int kPart = 32 * (DP + 4);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[d] *= scale;
+#pragma unroll
+        for (int n = 2; n > 0; n >>= 1) {
+            if (wave >= n && wave < 2 * n) {
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        *reinterpret_cast<f32x4*>(part + (wave - n) * kPart + at + 32 * d + 8 * x) =
+                            f32x4{o[d][4 * x], o[d][4 * x + 1], o[d][4 * x + 2], o[d][4 * x + 3]};
+            }
+            __syncthreads();
+            if (wave < n) {
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const f32x4 v = *reinterpret_cast<const f32x4*>(part + wave * kPart + at + 32 * d + 8 * x);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[d][4 * x + e] += v[e];
+                    }
+            }
+            __syncthreads();
+        }
+        if (wave != 0) return;
+    }
+    if (!live) return;
+
+    const int64_t row = (static_cast<int64_t>(b) * p.H + h) * p.Q + i;
+    if (sp.n > 1) {
+        const int64_t part = static_cast<int64_t>(split) * p.B * p.H * p.Q + row;
+        float* const to = sp.o + part * p.D;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int at = 32 * d + 8 * (e >> 2) + 4 * half + (e & 3);
+                if (at < p.D) to[at] = o[d][e];
+            }
+        if (half == 0) {
+            sp.ml[2 * part] = m;
+            sp.ml[2 * part + 1] = l;
+        }
+        return;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* const out = static_cast<T*>(p.out) + ((static_cast<int64_t>(b) * p.Q + i) * p.H + h) * p.D;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int at = 32 * d + 8 * x + 4 * half;
+            if (vec_out) {
+                typedef T T4 __attribute__((ext_vector_type(4)));
+                T4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(o[d][4 * x + e] * inv);
+                if (at < p.D) *reinterpret_cast<T4*>(out + at) = v;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (at + e < p.D) out[at + e] = static_cast<T>(o[d][4 * x + e] * inv);
+            }
+        }
+    if (p.stats != nullptr && half == 0) {
+        float* const st = static_cast<float*>(p.stats) + 2 * row;
+        st[0] = l == 0.f ? 0.f : m;
+        st[1] = l == 0.f ? 0.f : __builtin_amdgcn_logf(l) - kShift<T>;
+    }
+}
+
+// Joins the key ranges of each row: a wavefront a row, lanes over its channels.
+template <typename T>
+__global__ __launch_bounds__(64) void attn_join_kernel(AttnParams p, Split sp) {
+    const int lane = threadIdx.x;
+    const int64_t row = blockIdx.x, rows = static_cast<int64_t>(p.B) * p.H * p.Q;
+    float m = kNegInf;
+    for (int s = lane; s < sp.n; s += kWave) m = __builtin_fmaxf(m, sp.ml[2 * (s * rows + row)]);
+#pragma unroll
+    for (int x = 32; x > 0; x >>= 1) m = __builtin_fmaxf(m, xor_lane(m, x));
+    float l = 0.f;
+    for (int s = lane; s < sp.n; s += kWave) {
+        const float* ml = sp.ml + 2 * (s * rows + row);
+        if (ml[0] != kNegInf) l += ml[1] * __builtin_amdgcn_exp2f(ml[0] - m);
+    }
+    l = wave_sum(l);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int64_t i = row % p.Q, h = row / p.Q % p.H, b = row / p.Q / p.H;
+    T* const out = static_cast<T*>(p.out) + ((b * p.Q + i) * p.H + h) * p.D;
+    for (int d = lane; d < p.D; d += kWave) {
+        float o = 0.f;
+        for (int s = 0; s < sp.n; ++s) {
+            const int64_t part = s * rows + row;
+            const float ms = sp.ml[2 * part];
+            if (ms != kNegInf) o = fmaf(sp.o[part * p.D + d], __builtin_amdgcn_exp2f(ms - m), o);
+        }
+        out[d] = static_cast<T>(o * inv);
+    }
+    if (p.stats != nullptr && lane == 0) {
+        float* const st = static_cast<float*>(p.stats) + 2 * row;
+        st[0] = l == 0.f ? 0.f : m;
+        st[1] = l == 0.f ? 0.f : __builtin_amdgcn_logf(l) - kShift<T>;
+    }
+}
+
+// The launch shape. Workgroups of 128 rows that share key tiles, when they fill the GPU twice; else workgroups of 32 rows
+// with the keys over the wavefronts, and when those are few and the keys many, the keys over several workgroups too.
+struct Shape {
+    bool vec, wk;
+    int tiles, n, keys;
+};
+
+Shape shape_of(int dtype, const AttnParams& p) {
+    const int elem = elem_size(dtype);
+    auto ok = [&](const void* ptr, const int64_t (&s)[3]) {
+        return reinterpret_cast<uintptr_t>(ptr) % 16 == 0 && s[0] * elem % 16 == 0 && s[1] * elem % 16 == 0 &&
+               s[2] * elem % 16 == 0 && s[1] < (int64_t{1} << 31) / (64 * elem);
+    };
+    Shape s{};
+    s.vec = p.D * elem % 16 == 0 && ok(p.q, p.qs) && ok(p.k, p.ks) && ok(p.v, p.vs);
+    const int64_t heads = static_cast<int64_t>(p.B) * p.Hk;
+    const bool can = s.vec && padded_width(p.D) * elem <= 256;  // wider rows' private tiles do not fit in registers
+    s.wk = can && heads * ((p.rows + 127) / 128) < 512;
+    s.tiles = s.wk ? (p.rows + 31) / 32 : (p.rows + 127) / 128;
+    s.n = 1;
+    s.keys = p.K;
+    const int64_t groups = heads * s.tiles;
+    if (groups < 512 && p.K > 1024) {
+        int64_t n = (1024 + groups - 1) / groups;
+        const int64_t most = (p.K + 511) / 512;
+        n = n < most ? n : most;
+        const int64_t keys = ((p.K + n - 1) / n + 255) / 256 * 256;
+        s.keys = static_cast<int>(keys);
+        s.n = static_cast<int>((p.K + keys - 1) / keys);
+    }
+    return s;
+}
+
+template <typename T, int DP, bool WK, bool MASK, bool VEC>
+int run(const AttnParams& p, const Shape& s, const Split& sp, hipStream_t stream) {
+    static std::atomic<uint64_t> done{0};
+    constexpr int tile = 2 * key_tile<T, DP, WK>() * TileRows<T, DP>::kPitch;
+    constexpr int join = (256 + 2 * 32 * (DP + 4)) * 4;
+    constexpr int bytes = WK ? (4 * tile > join ? 4 * tile : join) : tile;
+    static_assert(bytes <= 160 * 1024, "LDS of a CU");
+    auto* const fn = &attn_forward_kernel<T, DP, WK, MASK, VEC>;
+    const hipError_t e =
+        bytes > 64 * 1024 ? allow_dynamic_lds(reinterpret_cast<const void*>(fn), bytes, done) : hipSuccess;
+    if (e != hipSuccess) return set_error(TD_E_LAUNCH, "attention: LDS size: %s", hipGetErrorString(e));
+    const int64_t n = static_cast<int64_t>(p.B) * p.Hk * s.tiles * s.n;
+    const bool vec_out = p.D % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % (4 * sizeof(T)) == 0;
+    hipLaunchKernelGGL(fn, dim3(xcd_grid(n)), dim3(256), bytes, stream, p, sp, vec_out, s.tiles);
+    if (s.n > 1)
+        hipLaunchKernelGGL((attn_join_kernel<T>), dim3(static_cast<unsigned>(p.B) * p.H * p.Q), dim3(64), 0, stream, p,
+                           sp);
+    const hipError_t le = hipGetLastError();
+    return le == hipSuccess ? 0 : set_error(TD_E_LAUNCH, "attention launch failed: %s", hipGetErrorString(le));
+}
+
+template <typename T, int DP>
+int run_dp(const AttnParams& p, const Shape& s, const Split& sp, hipStream_t stream) {
+    const bool mask = p.mask_type != TD_MASK_NONE;
+    if (!s.vec) return run<T, DP, false, true, false>(p, s, sp, stream);
+    if constexpr (DP * sizeof(T) <= 256)
+        if (s.wk)
+            return mask ? run<T, DP, true, true, true>(p, s, sp, stream)
+                        : run<T, DP, true, false, true>(p, s, sp, stream);
+    return mask ? run<T, DP, false, true, true>(p, s, sp, stream)
+                : run<T, DP, false, false, true>(p, s, sp, stream);
+}
+
+}  // namespace
+
+template <typename T>
+int launch_attn_forward_t(int dtype, const AttnParams& p, hipStream_t stream) {
+    const Shape s = shape_of(dtype, p);
+    const int64_t rows = static_cast<int64_t>(p.B) * p.H * p.Q;
+    const Split sp{s.n, s.keys, static_cast<float*>(p.ws), static_cast<float*>(p.ws) + s.n * rows * p.D};
+    switch (padded_width(p.D)) {
+        case 32: return run_dp<T, 32>(p, s, sp, stream);
+        case 64: return run_dp<T, 64>(p, s, sp, stream);
+        case 128: return run_dp<T, 128>(p, s, sp, stream);
+        default: return run_dp<T, 256>(p, s, sp, stream);
+    }
+}
+
+#if TD_ATTN_TYPE == 0
+template int launch_attn_forward_t<float>(int, const AttnParams&, hipStream_t);
+
+int64_t attn_forward_workspace(int dtype, const AttnParams& p) {
+    if (dtype == kF64) return 0;
+    const Shape s = shape_of(dtype, p);
+    return s.n == 1 ? 0 : static_cast<int64_t>(s.n) * p.B * p.H * p.Q * (p.D + 2) * 4;
+}
+
+int launch_attn_forward(int dtype, const AttnParams& p, hipStream_t stream) {
+    switch (dtype) {
+        case kF32: return launch_attn_forward_t<float>(dtype, p, stream);
+        case kF16: return launch_attn_forward_t<f16>(dtype, p, stream);
+        default: return launch_attn_forward_t<bf16>(dtype, p, stream);
+    }
+}
+#elif TD_ATTN_TYPE == 1
+template int launch_attn_forward_t<f16>(int, const AttnParams&, hipStream_t);
+#else
+template int launch_attn_forward_t<bf16>(int, const AttnParams&, hipStream_t);
+#endif
+
+}  // namespace td

@@ -1,0 +1,271 @@
+// Matrix-unit pieces of the attention kernels (td_attn_forward.hip, td_attn_backward.hip): 32 x 32 products of float32,
+// float16 and bfloat16 operands, and the tiles of keys or rows that they read from LDS.
+//
+// Every product is 32 x 32 with a float32 accumulator: element e of lane l is row 8 (e / 4) + 4 (l / 32) + e % 4 of
+// column l % 32. An operand is a fragment of 16 bytes a lane, l % 32 its row (or column) and l / 32 the half of a chunk
+// of 32 bytes of the inner dimension: 16 elements in 16 bits, 8 in float32. The order of the inner dimension is free as
+// long as both operands share it, which is what lets an accumulator be the next product's operand without leaving its
+// registers: a score tile's elements 8 s .. 8 s + 7 are the 16 rows 16 s .. 16 s + 15 of its column, in the order
+// (half, element) -> 16 s + 8 (element / 4) + 4 half + element % 4, and the other operand is read from LDS in that order.
+#pragma once
+
+#include <type_traits>
+
+#include "td_attn.h"
+
+namespace td {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef f16 f16x4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+struct Mma;
+template <>
+struct Mma<f16> {
+    __device__ __forceinline__ static f32x16 mul(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                      0, 0);
+    }
+};
+template <>
+struct Mma<bf16> {
+    __device__ __forceinline__ static f32x16 mul(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    }
+};
+template <>
+struct Mma<float> {
+    __device__ __forceinline__ static f32x16 mul(u32x4 a, u32x4 b, f32x16 c) {
+        const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i], y[i], c, 0, 0, 0);
+        return c;
+    }
+};
+
+// Rows of DP elements in LDS, 16 bytes longer than their data: with that pitch the 32 rows of a fragment read, the
+// transpose reads and the float32 column reads all go at the LDS's full rate (235 B/ns a CU, 118 and 109; without it
+// 131, 71 or 37 for rows of 64, 128 or 256 bytes, by a probe of the reads alone).
+template <typename T, int DP>
+struct TileRows {
+    static constexpr int kS = static_cast<int>(sizeof(T));
+    static constexpr int kPitch = DP * kS + 16;      // bytes
+    static constexpr int kChunks = DP * kS / 32;     // fragments of a row
+    static constexpr int kPieces = DP * kS / 16;     // 16-byte pieces of a row
+
+    // fragment `chunk` of rows row0 .. row0 + 31
+    __device__ __forceinline__ static u32x4 rows(const unsigned char* tile, int row0, int chunk, int lane) {
+        return *reinterpret_cast<const u32x4*>(tile + (row0 + (lane & 31)) * kPitch + chunk * 32 + (lane >> 5) * 16);
+    }
+
+    // acc += (columns d0 .. d0 + 31 of rows row0 .. row0 + 31)^T . w, with w a 32 x 32 tile over those rows in the
+    // accumulator's layout (16-bit: its elements rounded to T by pack()).
+    using Packed = std::conditional_t<sizeof(T) == 2, u32x4, f32x16>;
+    static constexpr int kPacked = sizeof(T) == 2 ? 2 : 1;
+    __device__ __forceinline__ static void pack(const f32x16& w, Packed (&o)[kPacked]) {
+        if constexpr (kS == 4) {
+            o[0] = w;
+        } else {
+            typedef T T8 __attribute__((ext_vector_type(8)));
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                T8 v;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = static_cast<T>(w[8 * s + j]);
+                o[s] = __builtin_bit_cast(u32x4, v);
+            }
+        }
+    }
+    __device__ __forceinline__ static f32x16 columns(const unsigned char* tile, int row0, int d0, int lane,
+                                                     const Packed (&w)[kPacked], f32x16 acc) {
+        if constexpr (kS == 4) {
+            const unsigned char* at = tile + (row0 + 4 * (lane >> 5)) * kPitch + (d0 + (lane & 31)) * 4;
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                acc = __builtin_amdgcn_mfma_f32_32x32x2f32(
+                    *reinterpret_cast<const float*>(at + (8 * (e >> 2) + (e & 3)) * kPitch), w[0][e], acc, 0, 0, 0);
+        } else {
+            // transpose reads: of 16 lanes, lane i points at row i / 4, columns 4 (i % 4) .. of a 4 x 16 block and
+            // receives its column i, the four rows
+            using v4s = short __attribute__((ext_vector_type(4)));
+            using lds_v4s = __attribute__((address_space(3))) v4s;
+            const int i = lane & 15;
+            const unsigned char* at = tile + (row0 + 4 * (lane >> 5) + (i >> 2)) * kPitch +
+                                      (d0 + 16 * ((lane >> 4) & 1) + 4 * (i & 3)) * 2;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 16 * s * kPitch));
+                const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + (16 * s + 8) * kPitch));
+                acc = Mma<T>::mul(__builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)),
+                                  w[s], acc);
+            }
+        }
+        return acc;
+    }
+};
+
+// 16 bytes of row `row` at byte `at` (a multiple of 16): zeros past the head's D elements. VEC: D * sizeof(T), the base
+// and every stride are multiples of 16 bytes, else element by element.
+template <typename T, bool VEC>
+__device__ __forceinline__ u32x4 row_piece(const T* row, int at, int D) {
+    constexpr int E = 16 / static_cast<int>(sizeof(T));
+    const int d = at / static_cast<int>(sizeof(T));
+    u32x4 r = {0u, 0u, 0u, 0u};
+    if constexpr (VEC) {
+        if (d < D) r = *reinterpret_cast<const u32x4*>(row + d);
+    } else {
+        typedef T TE __attribute__((ext_vector_type(E)));
+        TE v = __builtin_bit_cast(TE, r);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (d + e < D) v[e] = row[d + e];
+        r = __builtin_bit_cast(u32x4, v);
+    }
+    return r;
+}
+
+// NR rows of a tensor on their way to LDS through the registers of NT threads: rows whose bit in `gone` is set are
+// zeros and are not read. VEC as in row_piece, and NR rows span less than 2^31 bytes.
+template <typename T, int DP, int NR, int NT, bool VEC>
+struct StagedRows {
+    using R = TileRows<T, DP>;
+    static constexpr int kN = NR * R::kPieces / NT;  // pieces a thread
+    static_assert(NR <= 64 && NR * R::kPieces % NT == 0, "whole pieces for every thread");
+    u32x4 r[kN];
+    unsigned off[VEC ? kN : 1];  // bytes from the tile's first row
+
+    __device__ __forceinline__ static int row_of(int u, int t) { return (t + u * NT) / R::kPieces; }
+    __device__ __forceinline__ static int at_of(int u, int t) { return (t + u * NT) % R::kPieces * 16; }
+
+    // f(i): elements from the tile's first row to its row i
+    template <typename F>
+    __device__ __forceinline__ void plan(F f, int D, int t) {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int u = 0; u < kN; ++u) {
+                const int at = at_of(u, t);
+                off[u] = static_cast<unsigned>(f(row_of(u, t)) * R::kS) + (at < D * R::kS ? at : 0);
+            }
+        }
+    }
+    // base: the tile's first row; f as in plan
+    template <typename F>
+    __device__ __forceinline__ void load(const T* base, F f, uint64_t gone, int D, int t) {
+        if constexpr (VEC) {
+            const unsigned char* const bytes = reinterpret_cast<const unsigned char*>(base);
+            if (gone == 0) {
+#pragma unroll
+                for (int u = 0; u < kN; ++u) r[u] = *reinterpret_cast<const u32x4*>(bytes + off[u]);
+            } else {
+#pragma unroll
+                for (int u = 0; u < kN; ++u) {
+                    r[u] = u32x4{0u, 0u, 0u, 0u};
+                    if (!((gone >> row_of(u, t)) & 1)) r[u] = *reinterpret_cast<const u32x4*>(bytes + off[u]);
+                }
+            }
+            if (D < DP) {
+#pragma unroll
+                for (int u = 0; u < kN; ++u)
+                    if (at_of(u, t) >= D * R::kS) r[u] = u32x4{0u, 0u, 0u, 0u};
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < kN; ++u) {
+                const int row = row_of(u, t);
+                r[u] = u32x4{0u, 0u, 0u, 0u};
+                if (!((gone >> row) & 1)) r[u] = row_piece<T, false>(base + f(row), at_of(u, t), D);
+                __builtin_amdgcn_sched_barrier(0);  // one piece's loads at a time: all of them do not fit in registers
+            }
+        }
+    }
+    __device__ __forceinline__ void store(unsigned char* tile, int t) const {
+#pragma unroll
+        for (int u = 0; u < kN; ++u) *reinterpret_cast<u32x4*>(tile + row_of(u, t) * R::kPitch + at_of(u, t)) = r[u];
+    }
+};
+
+// Orders a wavefront's LDS accesses before it against those after it. The LDS serves one wavefront's accesses in order,
+// so this keeps the compiler from moving them and costs nothing.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Value of `v` in the lane 32 away
+__device__ __forceinline__ float other_half(float v) { return xor_lane(v, 32); }
+
+// The workgroup's place in the XCD-contiguous order: workgroup w runs on XCD w % 8, so that the `n` pieces of work in
+// order are dealt in eight contiguous runs and neighbours (tiles of one head, which read the same keys) share an L2.
+// Negative: no work.
+__device__ __forceinline__ int xcd_order(int w, int n) {
+    const int per = (n + kXcds - 1) / kXcds;
+    const int i = (w % kXcds) * per + w / kXcds;
+    return w / kXcds < per && i < n ? i : -1;
+}
+inline unsigned xcd_grid(int64_t n) { return static_cast<unsigned>((n + kXcds - 1) / kXcds * kXcds); }
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNegInf = -__builtin_inff();
+constexpr float kLowest = -3.4028234663852886e38f;
+
+// An additive mask's entry in base 2. The lowest float32 (and a mask below 2^127.5) keeps finite, so that a row of it
+// alone stays a uniform row, as in exact arithmetic with rounding to 24 bits; -inf stays -inf.
+__device__ __forceinline__ float mask_log2(float m) {
+    return m == kNegInf ? kNegInf : __builtin_fmaxf(m * kLog2e, kLowest);
+}
+
+// Four consecutive mask entries of a row at key j, `left` of them inside it
+template <typename T>
+__device__ __forceinline__ void mask4_float(const T* m, int left, bool whole, float (&o)[4]) {
+    T v[4];
+    if (whole) {
+        __builtin_memcpy(v, m, sizeof(v));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = e < left ? m[e] : static_cast<T>(0.f);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = mask_log2(static_cast<float>(v[e]));
+}
+__device__ __forceinline__ unsigned mask4_bytes(const uint8_t* m, int left, bool whole) {
+    unsigned v = 0;
+    if (whole) {
+        __builtin_memcpy(&v, m, 4);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < left) v |= static_cast<unsigned>(m[e]) << (8 * e);
+    }
+    return v;
+}
+
+// Scores of 32 keys (rows 8 i + 4 half + e) by 32 rows of the problem (columns), as the scores in base 2 with -inf where
+// a pair is left out: s *= c, plus the mask. `gone`: bit k set for key j0 + k that nobody sees (shifted by 4 half).
+// last: the last key that the lane's row sees (causal; INT32_MAX without). mrow: the mask's row (or null).
+template <typename T>
+__device__ __forceinline__ void mask_scores(f32x16& s, const AttnParams& p, int j0, unsigned gone, int last,
+                                            const void* mrow, int half, bool whole) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int j = j0 + 8 * i + 4 * half;
+        float add[4] = {0.f, 0.f, 0.f, 0.f};
+        unsigned bytes = 0;
+        if (mrow != nullptr) {
+            if (p.mask_type == TD_MASK_FLOAT)
+                mask4_float<T>(static_cast<const T*>(mrow) + j, p.K - j, whole, add);
+            else
+                bytes = mask4_bytes(static_cast<const uint8_t*>(mrow) + j, p.K - j, whole);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool out = ((gone >> (8 * i + e)) & 1u) || j + e > last || ((bytes >> (8 * e)) & 0xffu) ||
+                             add[e] == kNegInf;
+            const float t = fmaf(s[4 * i + e], p.c, add[e]);
+            s[4 * i + e] = out ? kNegInf : t;
+        }
+    }
+}
+
+}  // namespace td

@@ -64,10 +64,10 @@ def make_attn(size, dtype, mask='none', seed=0, grad_scale=1.0):
 def half_steps(dtype):
     """Half steps of dtype, of its accumulation type, and of P and dS (rounded to dtype where it has 16 bits), and what a
     probability may be off by where it is too small: the smallest normal number (an exponential below it may come out as
-    0), and in float16, whose P is held as 2^15 P with steps of 2^-24 where it is smallest, half such a step."""
+    0), and in float16, whose P is held as 2^11 P or more with steps of 2^-24 where it is smallest, half such a step."""
     u = torch.finfo(dtype).eps / 2
     a = u if dtype == torch.float64 else 2.0 ** -24
-    low = {torch.float64: 2.0 ** -1022, torch.float16: 2.0 ** -40}.get(dtype, 2.0 ** -126)
+    low = {torch.float64: 2.0 ** -1022, torch.float16: 2.0 ** -36}.get(dtype, 2.0 ** -126)
     return u, a, max(u, a), low
 
 

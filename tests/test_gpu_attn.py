@@ -268,3 +268,16 @@ def test_c_abi_writes_its_buffers_and_nothing_else(dtype):
             assert (whole[:fence] == 7).all() and (whole[fence + n:] == 7).all()
         check_attn(dtype, q.cpu(), k.cpu(), v.cpu(), go.cpu(), {}, out.view(B, Q, H * D),
                    (dq.view(q.shape), dk.view(k.shape), dv.view(v.shape)))
+
+
+def test_a_long_cache_past_32_bit_offsets():
+    # 4.5e9 elements of keys: rows behind the 2^32nd element are read through 64-bit offsets
+    K, Hk, D = 70_000_000, 1, 64
+    key = torch.zeros(1, K, Hk, D, dtype=torch.float16, device='cuda')
+    value = torch.zeros(1, K, Hk, D, dtype=torch.float16, device='cuda')
+    key[0, K - 3], value[0, K - 3] = 10, torch.arange(D, device='cuda').half()[None]
+    key[0, 1], value[0, 1] = 10, 1
+    q = torch.full((1, 1, 1, D), 10.0, dtype=torch.float16, device='cuda')  # scores 800 there, 0 elsewhere
+    out = td.ma_attn(q, key, value)
+    want = (torch.arange(D).double() + 1) / 2
+    agree(out.view(D), want.numpy(), want.numpy() * 2.0 ** -10, 1e-3, 'out')
