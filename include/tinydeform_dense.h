@@ -41,7 +41,7 @@ typedef struct td_attn_args {
     int32_t reserved; /* 0 */
     int64_t B, Q, K, H, Hk, D; /* Hk divides H; D <= TD_ATTN_MAX_HEAD_DIM; Q, K, B * Q * H, B * K * Hk <= INT32_MAX */
     double scale;              /* finite, > 0 */
-    const void* query;         /* [B, Q, H, D], element strides below (batch, token, head), the last one 1 */
+    const void* query;         /* [B, Q, H, D], element strides below (batch, token, head; not negative), the last one 1 */
     const void* key;           /* [B, K, Hk, D] */
     const void* value;         /* [B, K, Hk, D] */
     int64_t query_stride[3], key_stride[3], value_stride[3];

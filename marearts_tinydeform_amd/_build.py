@@ -28,10 +28,10 @@ ARCH = 'gfx950'
 
 SOURCES = ['td_abi.hip', 'td_fused.hip', 'td_sample.hip', 'td_gemm.hip', 'td_gemm_dma.hip', 'td_gemm_stream.hip',
            'td_gemm_split.hip', 'td_layer.hip', 'td_backward.hip', 'td_noalloc.hip', 'td_probe.hip', 'td_attn.hip',
-           'td_attn_forward.hip', 'td_norm.hip']
+           'td_attn_forward.hip', 'td_attn_backward.hip', 'td_norm.hip']
 
 # compiled once per element type (TD_ATTN_TYPE 0 float32, 1 float16, 2 bfloat16), so that the types build in parallel
-BY_TYPE = ['td_attn_forward.hip']
+BY_TYPE = ['td_attn_forward.hip', 'td_attn_backward.hip']
 
 # per-source additions: the direct-to-LDS GEMM keeps its MFMA accumulators in architectural VGPRs (in the
 # accumulator-register form the compiler copies every accumulator through a temporary in the inner loop)

@@ -38,6 +38,11 @@ int64_t attn_forward_workspace(int dtype, const AttnParams& p);
 int launch_attn_forward(int dtype, const AttnParams& p, hipStream_t stream);
 template <typename T>
 int launch_attn_forward_t(int dtype, const AttnParams& p, hipStream_t stream);
+// ... and the gradients (td_attn_backward.hip)
+int64_t attn_backward_workspace(int dtype, const AttnParams& p);
+int launch_attn_backward(int dtype, const AttnParams& p, hipStream_t stream);
+template <typename T>
+int launch_attn_backward_t(int dtype, const AttnParams& p, hipStream_t stream);
 // Head widths the matrix-unit kernels are built for
 inline int padded_width(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 

@@ -306,6 +306,9 @@ int check_args(const td_attn_args* a) {
     if (a->B > kIntMax || a->Q > kIntMax || a->K > kIntMax || a->H > kIntMax ||
         static_cast<__int128>(a->B) * a->Q * a->H > kIntMax || static_cast<__int128>(a->B) * a->K * a->Hk > kIntMax)
         return set_error(TD_E_ARG, "too many (batch, token, head) rows");
+    for (int i = 0; i < 3; ++i)
+        if (a->query_stride[i] < 0 || a->key_stride[i] < 0 || a->value_stride[i] < 0 || a->mask_stride[i] < 0)
+            return set_error(TD_E_ARG, "strides must be non-negative");
     if (!(a->scale > 0) || !isfinite(a->scale)) return set_error(TD_E_ARG, "scale must be positive and finite");
     if (a->mask_type < TD_MASK_NONE || a->mask_type > TD_MASK_FLOAT)
         return set_error(TD_E_ARG, "unknown mask type %d", a->mask_type);
@@ -351,7 +354,7 @@ extern "C" int td_attn_forward(const td_attn_args* args, void* workspace, int64_
 
 extern "C" int64_t td_attn_backward_workspace(const td_attn_args* args) {
     const int rc = check_args(args);
-    return rc != TD_OK ? rc : args->B * args->H * args->Q * (args->dtype == TD_F64 ? 8 : 4);
+    return rc != TD_OK ? rc : attn_backward_workspace(args->dtype, attn_params(*args));
 }
 
 extern "C" int td_attn_backward(const td_attn_args* args, const void* grad_out, void* grad_query, void* grad_key,
@@ -372,6 +375,7 @@ extern "C" int td_attn_backward(const td_attn_args* args, const void* grad_out, 
     p.dq = grad_query;
     p.dk = grad_key;
     p.dv = grad_value;
-    p.delta = workspace;
-    return launch_attn_backward_generic(args->dtype, p, static_cast<hipStream_t>(stream));
+    p.ws = p.delta = workspace;
+    if (args->dtype == TD_F64) return launch_attn_backward_generic(args->dtype, p, static_cast<hipStream_t>(stream));
+    return launch_attn_backward(args->dtype, p, static_cast<hipStream_t>(stream));
 }

@@ -1,0 +1,682 @@
+// Attention among tokens, backward, on the matrix units (float32, float16, bfloat16): the probabilities are computed again
+// from the scores and the forward's statistics, P = 2^(t - m - log2 l), and with g = grad_out
+//   dV = P^T g,  dP = g V^T,  dS = P (dP - delta),  delta = g . out,  dQ = scale dS K,  dK = scale dS^T Q.
+// Three launches: delta (and the statistics in the order of the problem's rows); dQ, a workgroup's rows against every key,
+// as the forward; dK and dV, a workgroup's keys against every row, so that no sum needs an atomic. That computes scores
+// and dP twice, 7 products where 5 would do; the other way, dQ summed over key blocks in memory, moves 4 D bytes for each
+// 32 D flops of a 128-key block's pairs and rows.
+#include "td_attn_mma.h"
+
+#ifndef TD_ATTN_TYPE
+#error "TD_ATTN_TYPE"
+#endif
+
+namespace td {
+namespace {
+
+// What the gradient kernels read of a row: m, log2 l, delta.
+struct RowInfo {
+    f32x4* rows;    // [B * Hk][rows]
+    float* amax;    // float16: [B * Hk][blocks] largest |g| of 64 rows, then [B * Hk][key_blocks] largest |v| of 64 keys
+    int blocks, key_blocks;
+};
+
+// float16 holds P as 2^15 P (normal numbers down to 2^-29) and dS as 2^15 P (dP - delta) 2^-e, e the exponent of
+// 2 D max|g| max|v| >= |dP - delta|: it cannot overflow, and a product 2^8 under that bound with a P of 2^-13 still has
+// all its bits. The other types have float32's exponents and need neither.
+template <typename T>
+constexpr bool kScaled = std::is_same<T, f16>::value;
+template <typename T>
+constexpr float kPShift = kScaled<T> ? 15.f : 0.f;
+
+constexpr int kInfoRows = 64;
+
+// 64 rows (or, in float16, the keys' values) a workgroup, four threads each
+template <typename T>
+__global__ __launch_bounds__(256) void attn_info_kernel(AttnParams p, RowInfo info, bool vec) {
+    __shared__ float best[4];
+    const int per = info.blocks + (kScaled<T> ? info.key_blocks : 0);
+    const int bh = blockIdx.x / per, block = blockIdx.x % per, b = bh / p.Hk, hk = bh % p.Hk;
+    const int t = threadIdx.x, part = t & 3;
+    constexpr int E = 16 / static_cast<int>(sizeof(T));
+    const bool is_row = block < info.blocks;
+    const int n = (is_row ? block : block - info.blocks) * kInfoRows + (t >> 2);
+    float top = 0.f;
+    auto see = [&](float v) {
+        const float a = __builtin_fabsf(v);
+        top = a < __builtin_inff() && a > top ? a : top;  // what is not finite shows in the results by itself
+    };
+    if (is_row) {
+        float delta = 0.f;
+        if (n < p.rows) {
+            const int i = static_cast<int>(fast_div(p.gdiv, n)), h = hk * p.G + n - i * p.G;
+            const int64_t at = ((static_cast<int64_t>(b) * p.Q + i) * p.H + h) * p.D;
+            const T *g = static_cast<const T*>(p.go) + at, *o = static_cast<const T*>(p.out) + at;
+            if (vec) {
+                for (int d = part * E; d < p.D; d += 4 * E) {
+                    float x[E], y[E];
+                    VecIO<T, E>::unpack(VecIO<T, E>::load(g + d), x);
+                    VecIO<T, E>::unpack(VecIO<T, E>::load(o + d), y);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        delta = fmaf(x[e], y[e], delta);
+                        see(x[e]);
+                    }
+                }
+            } else {
+                for (int d = part; d < p.D; d += 4) {
+                    delta = fmaf(static_cast<float>(g[d]), static_cast<float>(o[d]), delta);
+                    see(static_cast<float>(g[d]));
+                }
+            }
+            delta += xor_lane(delta, 1);
+            delta += xor_lane(delta, 2);
+            if (part == 0) {
+                const float* st =
+                    static_cast<const float*>(p.stats) + 2 * ((static_cast<int64_t>(b) * p.H + h) * p.Q + i);
+                info.rows[static_cast<int64_t>(bh) * p.rows + n] = f32x4{st[0], st[1], delta, 0.f};
+            }
+        }
+    } else if (n < p.K && (p.pad == nullptr || p.pad[static_cast<int64_t>(b) * p.K + n] == 0)) {
+        const T* v = static_cast<const T*>(p.v) + b * p.vs[0] + n * p.vs[1] + hk * p.vs[2];
+        for (int d = part; d < p.D; d += 4) see(static_cast<float>(v[d]));
+    }
+    if constexpr (kScaled<T>) {
+#pragma unroll
+        for (int x = 32; x > 0; x >>= 1) top = __builtin_fmaxf(top, xor_lane(top, x));
+        if (t % kWave == 0) best[t / kWave] = top;
+        __syncthreads();
+        if (t == 0) {
+            top = __builtin_fmaxf(__builtin_fmaxf(best[0], best[1]), __builtin_fmaxf(best[2], best[3]));
+            const int64_t heads = static_cast<int64_t>(p.B) * p.Hk;
+            if (is_row)
+                info.amax[static_cast<int64_t>(bh) * info.blocks + block] = top;
+            else
+                info.amax[heads * info.blocks + static_cast<int64_t>(bh) * info.key_blocks + block - info.blocks] = top;
+        }
+    }
+}
+
+// The power of two that dP - delta is multiplied by (float16), a wavefront's lanes together
+template <typename T>
+__device__ __forceinline__ float ds_factor(const AttnParams& p, const RowInfo& info, int bh, int lane) {
+    if constexpr (!kScaled<T>) return 1.f;
+    const float* g = info.amax + static_cast<int64_t>(bh) * info.blocks;
+    const float* v = info.amax + static_cast<int64_t>(p.B) * p.Hk * info.blocks +
+                     static_cast<int64_t>(bh) * info.key_blocks;
+    float a = 0.f, c = 0.f;
+    for (int i = lane; i < info.blocks; i += kWave) a = __builtin_fmaxf(a, g[i]);
+    for (int i = lane; i < info.key_blocks; i += kWave) c = __builtin_fmaxf(c, v[i]);
+#pragma unroll
+    for (int x = 32; x > 0; x >>= 1) {
+        a = __builtin_fmaxf(a, xor_lane(a, x));
+        c = __builtin_fmaxf(c, xor_lane(c, x));
+    }
+    // 2 D max|g| max|v| < 2^42: an exponent from the float's bits, and none below 2^-100 (nothing but zeros)
+    const unsigned u = __builtin_bit_cast(unsigned, __builtin_fmaxf(2.f * p.D * a * c, 0x1p-100f));
+    const unsigned e = (u >> 23) + 1;                      // the bound is below 2^(e - 127)
+    return __builtin_bit_cast(float, (254u - e) << 23);    // 2^(127 - e)
+}
+
+// dQ. The forward's shape: WK false, four wavefronts of 32 rows share the key tiles; WK true, 32 rows a workgroup and the
+// key tiles dealt to the wavefronts, whose sums are joined in LDS.
+template <typename T, int DP, bool WK>
+constexpr int dq_key_tile() {
+    return WK || DP * static_cast<int>(sizeof(T)) > 128 ? 32 : 64;
+}
+template <typename T, int DP, bool SLOW>
+constexpr int dq_min_waves() {
+    constexpr int bytes = DP * static_cast<int>(sizeof(T));
+    return bytes <= 64 ? (SLOW ? 2 : 3) : bytes <= 128 ? 2 : 1;
+}
+
+template <typename T, int DP, bool WK, bool MASK, bool VEC>
+__global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dq_kernel(AttnParams p, RowInfo info,
+                                                                                    bool vec_out, int tiles) {
+    using R = TileRows<T, DP>;
+    constexpr int KT = dq_key_tile<T, DP, WK>(), NT = WK ? 64 : 256, ND = DP / 32;
+    constexpr int kTile = KT * R::kPitch;
+    extern __shared__ __align__(16) unsigned char lds[];
+    const int id = xcd_order(static_cast<int>(blockIdx.x), p.B * p.Hk * tiles);
+    if (id < 0) return;
+    const int tile = tiles - 1 - id % tiles, bh = id / tiles;  // causal: the long ones first
+    const int b = bh / p.Hk, hk = bh % p.Hk;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    const int lane = threadIdx.x % kWave, half = lane >> 5;
+    const int t = WK ? lane : static_cast<int>(threadIdx.x);
+    unsigned char* const kt_lds = lds + (WK ? wave * 2 * kTile : 0);
+    unsigned char* const vt_lds = kt_lds + kTile;
+
+    const int row0 = tile * (WK ? 32 : 128), wrow0 = row0 + (WK ? 0 : wave * 32), r = wrow0 + (lane & 31);
+    const bool live = r < p.rows;
+    const int i = static_cast<int>(fast_div(p.gdiv, static_cast<uint32_t>(live ? r : 0)));
+    const int h = hk * p.G + (live ? r : 0) - i * p.G;
+    const int64_t out_at = ((static_cast<int64_t>(b) * p.Q + i) * p.H + h) * p.D;
+    u32x4 qf[R::kChunks], gf[R::kChunks];
+    {
+        const T* q = static_cast<const T*>(p.q) + b * p.qs[0] + i * p.qs[1] + h * p.qs[2];
+        const T* g = static_cast<const T*>(p.go) + out_at;
+#pragma unroll
+        for (int c = 0; c < R::kChunks; ++c) {
+            qf[c] = live ? row_piece<T, VEC>(q, c * 32 + half * 16, p.D) : u32x4{0u, 0u, 0u, 0u};
+            gf[c] = live ? row_piece<T, VEC>(g, c * 32 + half * 16, p.D) : u32x4{0u, 0u, 0u, 0u};
+        }
+    }
+    const f32x4 ri = info.rows[static_cast<int64_t>(bh) * p.rows + (live ? r : 0)];
+    const float ds_scale = ds_factor<T>(p, info, bh, lane);
+    const float delta = ri[2] * ds_scale;
+    const unsigned char* const mrow =
+        !MASK ? nullptr
+              : static_cast<const unsigned char*>(p.mask) + (b * p.ms[0] + h * p.ms[1] + i * p.ms[2]) *
+                                                                (p.mask_type == TD_MASK_FLOAT ? sizeof(T) : 1);
+    // an additive mask may make m so large that log2 l is lost beside it: it is subtracted after t - m then
+    const bool apart = MASK && p.mask_type == TD_MASK_FLOAT;
+    const float from = apart ? ri[0] : ri[0] + ri[1] - kPShift<T>, then = apart ? ri[1] - kPShift<T> : 0.f;
+    const int diag = static_cast<int>(p.diag);
+    const int last = p.causal ? i + diag : 2147483647;
+    int kend = p.K;
+    const int top_row = (row0 + (WK ? 32 : 128) < p.rows ? row0 + (WK ? 32 : 128) : p.rows) - 1;
+    if (p.causal) {
+        const int seen = static_cast<int>(fast_div(p.gdiv, static_cast<uint32_t>(top_row))) + diag + 1;
+        kend = seen < kend ? seen : kend;
+    }
+    const int wtop = wrow0 + 31 < p.rows ? wrow0 + 31 : p.rows - 1;
+    const int wfirst = wrow0 < p.rows ? wrow0 : p.rows - 1;
+    const int seen_all = p.causal ? static_cast<int>(fast_div(p.gdiv, static_cast<uint32_t>(wfirst))) + diag : 2147483647;
+    const int seen_any = p.causal ? static_cast<int>(fast_div(p.gdiv, static_cast<uint32_t>(wtop))) + diag : 2147483647;
+
+    const T* const kb = static_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[2];
+    const T* const vb = static_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[2];
+    const uint8_t* const pad = p.pad == nullptr ? nullptr : p.pad + static_cast<int64_t>(b) * p.K;
+    auto pad_byte = [&](int64_t j0) -> int {
+        const int64_t j = j0 + lane;
+        return lane >= KT || j >= kend || (pad != nullptr && pad[j] != 0);
+    };
+    StagedRows<T, DP, KT, NT, VEC> ks, vs;
+    auto k_row = [&](int x) { return x * p.ks[1]; };
+    auto v_row = [&](int x) { return x * p.vs[1]; };
+    ks.plan(k_row, p.D, t);
+    vs.plan(v_row, p.D, t);
+    f32x16 dq[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) dq[d] = f32x16{0.f};
+
+    constexpr int step = WK ? 4 * KT : KT;
+    constexpr uint64_t all = KT == 64 ? ~uint64_t{0} : (uint64_t{1} << (KT & 63)) - 1;
+    int64_t j0 = WK ? wave * KT : 0;
+    uint64_t gone = __ballot(pad_byte(j0)), gone_next;
+    auto fetch = [&](int64_t at, uint64_t g) {
+        ks.load(kb + at * p.ks[1], k_row, g & all, p.D, t);
+        vs.load(vb + at * p.vs[1], v_row, g & all, p.D, t);
+    };
+    if (j0 < kend) fetch(j0, gone);
+    int next_pad = pad_byte(j0 + step);
+    for (; j0 < kend; j0 += step) {
+        if (!WK) __syncthreads();
+        ks.store(kt_lds, t);
+        vs.store(vt_lds, t);
+        if (WK)
+            wave_sync();
+        else
+            __syncthreads();
+        gone_next = __ballot(next_pad);
+        if (j0 + step < kend) {
+            fetch(j0 + step, gone_next);
+            next_pad = pad_byte(j0 + 2 * step);
+        }
+        const int j = static_cast<int>(j0);
+        if ((gone & all) != all && j <= seen_any) {
+            const bool whole = j + KT <= p.K;
+            const bool masked = (gone & all) != 0 || mrow != nullptr || j + KT - 1 > seen_all;
+#pragma unroll
+            for (int x = 0; x < KT / 32; ++x) {
+                f32x16 s = f32x16{0.f}, dp = f32x16{0.f};
+#pragma unroll
+                for (int c = 0; c < R::kChunks; ++c) {
+                    s = Mma<T>::mul(R::rows(kt_lds, 32 * x, c, lane), qf[c], s);
+                    dp = Mma<T>::mul(R::rows(vt_lds, 32 * x, c, lane), gf[c], dp);
+                }
+                float cc = p.c;
+                if (masked) {
+                    cc = 1.f;
+                    mask_scores<T>(s, p, j + 32 * x, static_cast<unsigned>(gone >> (32 * x + 4 * half)), last, mrow, half,
+                                   whole);
+                }
+                f32x16 ds;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    float y = fmaf(s[e], cc, -from);
+                    if (apart) y -= then;
+                    ds[e] = __builtin_amdgcn_exp2f(y) * fmaf(dp[e], ds_scale, -delta);
+                }
+                typename R::Packed w[R::kPacked];
+                R::pack(ds, w);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) dq[d] = R::columns(kt_lds, 32 * x, 32 * d, lane, w, dq[d]);
+            }
+        }
+        gone = gone_next;
+        if (WK) wave_sync();
+    }
+    if constexpr (WK) {
+        float* const part = reinterpret_cast<float*>(lds);
+        const int at = (lane & 31) * (DP + 4) + 4 * half;
+        constexpr int kPart = 32 * (DP + 4);
+        __syncthreads();
+#pragma unroll
+        for (int n = 2; n > 0; n >>= 1) {
+            if (wave >= n && wave < 2 * n) {
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        *reinterpret_cast<f32x4*>(part + (wave - n) * kPart + at + 32 * d + 8 * x) =
+                            f32x4{dq[d][4 * x], dq[d][4 * x + 1], dq[d][4 * x + 2], dq[d][4 * x + 3]};
+            }
+            __syncthreads();
+            if (wave < n) {
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const f32x4 v = *reinterpret_cast<const f32x4*>(part + wave * kPart + at + 32 * d + 8 * x);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) dq[d][4 * x + e] += v[e];
+                    }
+            }
+            __syncthreads();
+        }
+        if (wave != 0) return;
+    }
+    if (!live) return;
+    const float back = static_cast<float>(p.scale) / ds_scale * (kScaled<T> ? 0x1p-15f : 1.f);
+    T* const out = static_cast<T*>(p.dq) + out_at;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) store4<T>(out, 32 * d + 8 * x + 4 * half, p.D, vec_out, dq[d], 4 * x, back);
+}
+
+// dK and dV. WK false: four wavefronts of 32 keys each share the row tiles. WK true: 32 keys a workgroup and the row tiles
+// dealt to the wavefronts. The scores stand untransposed here (a lane's column is its key), so that P and dS are operands
+// of dV^T = g^T P and dK^T = Q^T dS as they stand. Rows past the end hold zeros and m = inf: P = 0.
+template <typename T, int DP, bool WK>
+constexpr int dkv_row_tile() {
+    return WK || DP * static_cast<int>(sizeof(T)) > 128 ? 32 : 64;
+}
+
+template <typename T, int DP, bool WK, bool MASK, bool VEC>
+__global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dkv_kernel(AttnParams p, RowInfo info,
+                                                                                     bool vec_out, int tiles) {
+    using R = TileRows<T, DP>;
+    constexpr int RT = dkv_row_tile<T, DP, WK>(), NT = WK ? 64 : 256, ND = DP / 32;
+    constexpr int kTile = RT * R::kPitch;
+    constexpr int kArea = 2 * kTile + RT * 24;  // two tiles, m and delta (or m, log2 l, delta) and mask offsets of the rows
+    extern __shared__ __align__(16) unsigned char lds[];
+    const int id = xcd_order(static_cast<int>(blockIdx.x), p.B * p.Hk * tiles);
+    if (id < 0) return;
+    const int tile = id % tiles, bh = id / tiles;  // causal: the first keys are seen by the most rows
+    const int b = bh / p.Hk, hk = bh % p.Hk;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    const int lane = threadIdx.x % kWave, half = lane >> 5;
+    const int t = WK ? lane : static_cast<int>(threadIdx.x);
+    unsigned char* const q_lds = lds + (WK ? wave * kArea : 0);
+    unsigned char* const g_lds = q_lds + kTile;
+    float* const m_lds = reinterpret_cast<float*>(g_lds + kTile);
+    float* const l_lds = m_lds + RT;
+    float* const d_lds = l_lds + RT;
+    int64_t* const o_lds = reinterpret_cast<int64_t*>(d_lds + RT);  // 12 RT bytes on: a multiple of 8
+
+    // the lane's key
+    const int key0 = tile * (WK ? 32 : 128), wkey0 = key0 + (WK ? 0 : wave * 32), j = wkey0 + (lane & 31);
+    const bool live = j < p.K && (p.pad == nullptr || p.pad[static_cast<int64_t>(b) * p.K + j] == 0);
+    u32x4 kf[R::kChunks], vf[R::kChunks];
+    {
+        const T* k = static_cast<const T*>(p.k) + b * p.ks[0] + j * p.ks[1] + hk * p.ks[2];
+        const T* v = static_cast<const T*>(p.v) + b * p.vs[0] + j * p.vs[1] + hk * p.vs[2];
+#pragma unroll
+        for (int c = 0; c < R::kChunks; ++c) {
+            kf[c] = live ? row_piece<T, VEC>(k, c * 32 + half * 16, p.D) : u32x4{0u, 0u, 0u, 0u};
+            vf[c] = live ? row_piece<T, VEC>(v, c * 32 + half * 16, p.D) : u32x4{0u, 0u, 0u, 0u};
+        }
+    }
+    const float ds_scale = ds_factor<T>(p, info, bh, lane);
+    const bool apart = MASK && p.mask_type == TD_MASK_FLOAT;
+    const int diag = static_cast<int>(p.diag);
+    const int mask_key = j < p.K ? j : p.K - 1;
+
+    // rows that see any of the workgroup's keys (or the wavefront's): query >= key - diag
+    int64_t r0 = 0;
+    const int first_q = key0 - diag > 0 ? key0 - diag : 0, wfirst_q = wkey0 - diag > 0 ? wkey0 - diag : 0;
+    if (p.causal) r0 = static_cast<int64_t>(first_q) * p.G / RT * RT;
+    const int64_t wfirst_row = p.causal ? static_cast<int64_t>(wfirst_q) * p.G : 0;
+    // from this row on every key of the wavefront is seen
+    const int64_t whole_row = p.causal ? (static_cast<int64_t>(wkey0) + 31 - diag) * p.G : 0;
+    const bool any = __any(live);
+
+    const T* const qb = static_cast<const T*>(p.q) + b * p.qs[0] + hk * p.G * p.qs[2];
+    const int64_t gs1 = static_cast<int64_t>(p.H) * p.D, gs2 = p.D;
+    const T* const gb = static_cast<const T*>(p.go) + b * p.Q * gs1 + hk * p.G * gs2;
+    const f32x4* const ib = info.rows + static_cast<int64_t>(bh) * p.rows;
+    StagedRows<T, DP, RT, NT, VEC> qs, gs;
+    // rows of a tile lie the same in every tile when the heads of a key head divide it
+    const bool even = RT % p.G == 0;
+    int64_t from_row = 0;
+    auto split_row = [&](int x, int& i, int& g) {
+        const uint32_t r = static_cast<uint32_t>(from_row + x);
+        i = static_cast<int>(fast_div(p.gdiv, r));
+        g = static_cast<int>(r) - i * p.G;
+        i -= static_cast<int>(fast_div(p.gdiv, static_cast<uint32_t>(from_row)));
+    };
+    auto q_row = [&](int x) {
+        int i, g;
+        split_row(x, i, g);
+        return i * p.qs[1] + g * p.qs[2];
+    };
+    auto g_row = [&](int x) {
+        int i, g;
+        split_row(x, i, g);
+        return i * gs1 + g * gs2;
+    };
+    if (even) {
+        qs.plan(q_row, p.D, t);
+        gs.plan(g_row, p.D, t);
+    }
+    f32x4 ri = f32x4{0.f, 0.f, 0.f, 0.f};
+    int64_t mo = 0;
+    auto fetch = [&](int64_t at) {
+        from_row = at;
+        const int64_t left = p.rows - at;
+        const uint64_t gone = left >= RT ? 0 : ~uint64_t{0} << left;
+        if (!even) {
+            qs.plan(q_row, p.D, t);
+            gs.plan(g_row, p.D, t);
+        }
+        const int64_t i0 = fast_div(p.gdiv, static_cast<uint32_t>(at));
+        qs.load(qb + i0 * p.qs[1], q_row, gone, p.D, t);
+        gs.load(gb + i0 * gs1, g_row, gone, p.D, t);
+        if (t < RT) {
+            const bool in = t < left;
+            ri = in ? ib[at + t] : f32x4{__builtin_inff(), 0.f, 0.f, 0.f};
+            if (MASK) {
+                const int i = static_cast<int>(fast_div(p.gdiv, static_cast<uint32_t>(in ? at + t : 0)));
+                const int g = static_cast<int>(in ? at + t : 0) - i * p.G;
+                mo = b * p.ms[0] + (hk * p.G + g) * p.ms[1] + i * p.ms[2];
+            }
+        }
+    };
+    f32x16 dk[ND], dv[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f32x16{0.f};
+
+    constexpr int step = WK ? 4 * RT : RT;
+    if (WK) r0 += wave * RT;
+    if (r0 < p.rows) fetch(r0);
+    for (; r0 < p.rows; r0 += step) {
+        if (!WK) __syncthreads();
+        qs.store(q_lds, t);
+        gs.store(g_lds, t);
+        if (t < RT) {
+            m_lds[t] = apart ? ri[0] : ri[0] + ri[1] - kPShift<T>;
+            l_lds[t] = ri[1] - kPShift<T>;
+            d_lds[t] = ri[2] * ds_scale;
+            if (MASK) o_lds[t] = mo;
+        }
+        if (WK)
+            wave_sync();
+        else
+            __syncthreads();
+        if (r0 + step < p.rows) fetch(r0 + step);
+        if (any && r0 + RT > wfirst_row) {
+            const bool masked = MASK || r0 < whole_row;
+#pragma unroll
+            for (int x = 0; x < RT / 32; ++x) {
+                f32x16 s = f32x16{0.f}, dp = f32x16{0.f};
+#pragma unroll
+                for (int c = 0; c < R::kChunks; ++c) {
+                    s = Mma<T>::mul(R::rows(q_lds, 32 * x, c, lane), kf[c], s);
+                    dp = Mma<T>::mul(R::rows(g_lds, 32 * x, c, lane), vf[c], dp);
+                }
+                float cc = p.c;
+                if (masked) {
+                    cc = 1.f;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int row = 32 * x + 8 * (e >> 2) + 4 * half + (e & 3);
+                        bool out = false;
+                        float add = 0.f;
+                        if (MASK && p.mask_type == TD_MASK_FLOAT) {
+                            add = mask_log2(static_cast<float>(static_cast<const T*>(p.mask)[o_lds[row] + mask_key]));
+                            out = add == kNegInf;
+                        } else if (MASK && p.mask_type == TD_MASK_BYTES) {
+                            out = static_cast<const uint8_t*>(p.mask)[o_lds[row] + mask_key] != 0;
+                        }
+                        if (p.causal)
+                            out |= j > static_cast<int>(fast_div(p.gdiv, static_cast<uint32_t>(r0 + row))) + diag;
+                        s[e] = out ? kNegInf : fmaf(s[e], p.c, add);
+                    }
+                }
+                f32x16 ds;
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const int row = 32 * x + 8 * y + 4 * half;
+                    const f32x4 m4 = *reinterpret_cast<const f32x4*>(m_lds + row);
+                    const f32x4 d4 = *reinterpret_cast<const f32x4*>(d_lds + row);
+                    f32x4 l4 = f32x4{0.f, 0.f, 0.f, 0.f};
+                    if (apart) l4 = *reinterpret_cast<const f32x4*>(l_lds + row);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float z = fmaf(s[4 * y + e], cc, -m4[e]);
+                        if (apart) z -= l4[e];
+                        const float pr = __builtin_amdgcn_exp2f(z);
+                        s[4 * y + e] = pr;
+                        ds[4 * y + e] = pr * fmaf(dp[4 * y + e], ds_scale, -d4[e]);
+                    }
+                }
+                typename R::Packed w[R::kPacked];
+                R::pack(s, w);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) dv[d] = R::columns(g_lds, 32 * x, 32 * d, lane, w, dv[d]);
+                R::pack(ds, w);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) dk[d] = R::columns(q_lds, 32 * x, 32 * d, lane, w, dk[d]);
+            }
+        }
+        if (WK) wave_sync();
+    }
+    if constexpr (WK) {
+        float* const part = reinterpret_cast<float*>(lds);
+        const int at = (lane & 31) * (DP + 4) + 4 * half;
+        constexpr int kPart = 32 * (DP + 4);
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            f32x16(&sum)[ND] = which ? dv : dk;
+            __syncthreads();
+#pragma unroll
+            for (int n = 2; n > 0; n >>= 1) {
+                if (wave >= n && wave < 2 * n) {
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+                            *reinterpret_cast<f32x4*>(part + (wave - n) * kPart + at + 32 * d + 8 * x) =
+                                f32x4{sum[d][4 * x], sum[d][4 * x + 1], sum[d][4 * x + 2], sum[d][4 * x + 3]};
+                }
+                __syncthreads();
+                if (wave < n) {
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const f32x4 v = *reinterpret_cast<const f32x4*>(part + wave * kPart + at + 32 * d + 8 * x);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) sum[d][4 * x + e] += v[e];
+                        }
+                }
+                __syncthreads();
+            }
+        }
+        if (wave != 0) return;
+    }
+    if (j >= p.K) return;
+    const float pv = live ? (kScaled<T> ? 0x1p-15f : 1.f) : 0.f;
+    const float back = static_cast<float>(p.scale) / ds_scale * (kScaled<T> ? 0x1p-15f : 1.f);
+    const int64_t at = ((static_cast<int64_t>(b) * p.K + j) * p.Hk + hk) * p.D;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+        if (!live) dk[d] = dv[d] = f32x16{0.f};  // a key that nobody sees: its column may hold anything
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int c = 32 * d + 8 * x + 4 * half;
+            store4<T>(static_cast<T*>(p.dk) + at, c, p.D, vec_out, dk[d], 4 * x, back);
+            store4<T>(static_cast<T*>(p.dv) + at, c, p.D, vec_out, dv[d], 4 * x, pv);
+        }
+    }
+}
+
+struct BackShape {
+    bool vec, wk_q, wk_k;
+    int q_tiles, k_tiles;
+};
+
+BackShape back_shape(int dtype, const AttnParams& p) {
+    const int elem = elem_size(dtype);
+    auto ok = [&](const void* ptr, const int64_t (&s)[3]) {
+        return reinterpret_cast<uintptr_t>(ptr) % 16 == 0 && s[0] * elem % 16 == 0 && s[1] * elem % 16 == 0 &&
+               s[2] * elem % 16 == 0 && s[1] < (int64_t{1} << 31) / (128 * elem) &&
+               s[2] < (int64_t{1} << 31) / (int64_t{2} * p.G * elem);
+    };
+    BackShape s{};
+    s.vec = p.D * elem % 16 == 0 && ok(p.q, p.qs) && ok(p.k, p.ks) && ok(p.v, p.vs) &&
+            reinterpret_cast<uintptr_t>(p.go) % 16 == 0 &&
+            static_cast<int64_t>(p.H) * p.D < (int64_t{1} << 31) / (128 * elem);
+    const int64_t heads = static_cast<int64_t>(p.B) * p.Hk;
+    const bool can = s.vec && padded_width(p.D) * elem <= 256;
+    s.wk_q = can && heads * ((p.rows + 127) / 128) < 512;
+    s.wk_k = can && heads * ((p.K + 127) / 128) < 512;
+    s.q_tiles = s.wk_q ? (p.rows + 31) / 32 : (p.rows + 127) / 128;
+    s.k_tiles = s.wk_k ? (p.K + 31) / 32 : (p.K + 127) / 128;
+    return s;
+}
+
+template <typename T, int DP, bool WK, bool MASK, bool VEC>
+int run_dq(const AttnParams& p, const BackShape& s, const RowInfo& info, hipStream_t stream) {
+    static std::atomic<uint64_t> done{0};
+    constexpr int tile = 2 * dq_key_tile<T, DP, WK>() * TileRows<T, DP>::kPitch;
+    constexpr int join = 2 * 32 * (DP + 4) * 4;
+    constexpr int bytes = WK ? (4 * tile > join ? 4 * tile : join) : tile;
+    static_assert(bytes <= 160 * 1024, "LDS of a CU");
+    auto* const fn = &attn_dq_kernel<T, DP, WK, MASK, VEC>;
+    const hipError_t e =
+        bytes > 64 * 1024 ? allow_dynamic_lds(reinterpret_cast<const void*>(fn), bytes, done) : hipSuccess;
+    if (e != hipSuccess) return set_error(TD_E_LAUNCH, "attention backward: LDS size: %s", hipGetErrorString(e));
+    const bool vec_out = p.D % 4 == 0 && reinterpret_cast<uintptr_t>(p.dq) % (4 * sizeof(T)) == 0;
+    const int64_t n = static_cast<int64_t>(p.B) * p.Hk * s.q_tiles;
+    hipLaunchKernelGGL(fn, dim3(xcd_grid(n)), dim3(256), bytes, stream, p, info, vec_out, s.q_tiles);
+    return 0;
+}
+
+template <typename T, int DP, bool WK, bool MASK, bool VEC>
+int run_dkv(const AttnParams& p, const BackShape& s, const RowInfo& info, hipStream_t stream) {
+    static std::atomic<uint64_t> done{0};
+    constexpr int RT = dkv_row_tile<T, DP, WK>(), area = 2 * RT * TileRows<T, DP>::kPitch + RT * 24;
+    constexpr int join = 2 * 32 * (DP + 4) * 4;
+    constexpr int bytes = WK ? (4 * area > join ? 4 * area : join) : area;
+    static_assert(bytes <= 160 * 1024, "LDS of a CU");
+    auto* const fn = &attn_dkv_kernel<T, DP, WK, MASK, VEC>;
+    const hipError_t e =
+        bytes > 64 * 1024 ? allow_dynamic_lds(reinterpret_cast<const void*>(fn), bytes, done) : hipSuccess;
+    if (e != hipSuccess) return set_error(TD_E_LAUNCH, "attention backward: LDS size: %s", hipGetErrorString(e));
+    const bool vec_out = p.D % 4 == 0 && reinterpret_cast<uintptr_t>(p.dk) % (4 * sizeof(T)) == 0 &&
+                         reinterpret_cast<uintptr_t>(p.dv) % (4 * sizeof(T)) == 0;
+    const int64_t n = static_cast<int64_t>(p.B) * p.Hk * s.k_tiles;
+    hipLaunchKernelGGL(fn, dim3(xcd_grid(n)), dim3(256), bytes, stream, p, info, vec_out, s.k_tiles);
+    return 0;
+}
+
+template <typename T, int DP>
+int run_dp(const AttnParams& p, const BackShape& s, const RowInfo& info, hipStream_t stream) {
+    const bool mask = p.mask_type != TD_MASK_NONE && p.K > 0;
+    int rc = 0;
+    if (p.dq != nullptr && p.rows > 0) {
+        if (!s.vec)
+            rc = mask ? run_dq<T, DP, false, true, false>(p, s, info, stream)
+                      : run_dq<T, DP, false, false, false>(p, s, info, stream);
+        else if (!s.wk_q)
+            rc = mask ? run_dq<T, DP, false, true, true>(p, s, info, stream)
+                      : run_dq<T, DP, false, false, true>(p, s, info, stream);
+        else if constexpr (DP * sizeof(T) <= 256)
+            rc = mask ? run_dq<T, DP, true, true, true>(p, s, info, stream)
+                      : run_dq<T, DP, true, false, true>(p, s, info, stream);
+    }
+    if (rc == 0 && p.dk != nullptr && p.K > 0) {
+        if (!s.vec)
+            rc = mask ? run_dkv<T, DP, false, true, false>(p, s, info, stream)
+                      : run_dkv<T, DP, false, false, false>(p, s, info, stream);
+        else if (!s.wk_k)
+            rc = mask ? run_dkv<T, DP, false, true, true>(p, s, info, stream)
+                      : run_dkv<T, DP, false, false, true>(p, s, info, stream);
+        else if constexpr (DP * sizeof(T) <= 256)
+            rc = mask ? run_dkv<T, DP, true, true, true>(p, s, info, stream)
+                      : run_dkv<T, DP, true, false, true>(p, s, info, stream);
+    }
+    return rc;
+}
+
+RowInfo info_of(const AttnParams& p) {
+    RowInfo r{};
+    r.rows = static_cast<f32x4*>(p.ws);
+    r.amax = reinterpret_cast<float*>(r.rows + static_cast<int64_t>(p.B) * p.Hk * p.rows);
+    r.blocks = (p.rows + kInfoRows - 1) / kInfoRows;
+    r.key_blocks = (p.K + kInfoRows - 1) / kInfoRows;
+    return r;
+}
+
+}  // namespace
+
+template <typename T>
+int launch_attn_backward_t(int dtype, const AttnParams& p, hipStream_t stream) {
+    const BackShape s = back_shape(dtype, p);
+    const RowInfo info = info_of(p);
+    const int64_t blocks =
+        static_cast<int64_t>(p.B) * p.Hk * (info.blocks + (kScaled<T> ? info.key_blocks : 0));
+    const bool vec = p.D * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(p.go) % 16 == 0 &&
+                     reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
+    if (blocks > 0)
+        hipLaunchKernelGGL((attn_info_kernel<T>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, p, info, vec);
+    int rc;
+    switch (padded_width(p.D)) {
+        case 32: rc = run_dp<T, 32>(p, s, info, stream); break;
+        case 64: rc = run_dp<T, 64>(p, s, info, stream); break;
+        case 128: rc = run_dp<T, 128>(p, s, info, stream); break;
+        default: rc = run_dp<T, 256>(p, s, info, stream);
+    }
+    if (rc != 0) return rc;
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? 0 : set_error(TD_E_LAUNCH, "attention backward launch failed: %s", hipGetErrorString(e));
+}
+
+#if TD_ATTN_TYPE == 0
+template int launch_attn_backward_t<float>(int, const AttnParams&, hipStream_t);
+
+int64_t attn_backward_workspace(int dtype, const AttnParams& p) {
+    const int64_t rows = static_cast<int64_t>(p.B) * p.H * p.Q;
+    if (dtype == kF64) return rows * 8;
+    const RowInfo r = info_of(p);
+    return rows * 16 + (dtype == kF16 ? static_cast<int64_t>(p.B) * p.Hk * (r.blocks + r.key_blocks) * 4 : 0);
+}
+
+int launch_attn_backward(int dtype, const AttnParams& p, hipStream_t stream) {
+    switch (dtype) {
+        case kF32: return launch_attn_backward_t<float>(dtype, p, stream);
+        case kF16: return launch_attn_backward_t<f16>(dtype, p, stream);
+        default: return launch_attn_backward_t<bf16>(dtype, p, stream);
+    }
+}
+#elif TD_ATTN_TYPE == 1
+template int launch_attn_backward_t<f16>(int, const AttnParams&, hipStream_t);
+#else
+template int launch_attn_backward_t<bf16>(int, const AttnParams&, hipStream_t);
+#endif
+
+}  // namespace td

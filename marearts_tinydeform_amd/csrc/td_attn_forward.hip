@@ -270,20 +270,7 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const int at = 32 * d + 8 * x + 4 * half;
-            if (vec_out) {
-                typedef T T4 __attribute__((ext_vector_type(4)));
-                T4 v;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(o[d][4 * x + e] * inv);
-                if (at < p.D) *reinterpret_cast<T4*>(out + at) = v;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (at + e < p.D) out[at + e] = static_cast<T>(o[d][4 * x + e] * inv);
-            }
-        }
+        for (int x = 0; x < 4; ++x) store4<T>(out, 32 * d + 8 * x + 4 * half, p.D, vec_out, o[d], 4 * x, inv);
     if (p.stats != nullptr && half == 0) {
         float* const st = static_cast<float*>(p.stats) + 2 * row;
         st[0] = l == 0.f ? 0.f : m;

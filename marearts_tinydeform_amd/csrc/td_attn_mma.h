@@ -241,6 +241,22 @@ __device__ __forceinline__ unsigned mask4_bytes(const uint8_t* m, int left, bool
     return v;
 }
 
+// Elements x .. x + 3 of an accumulator, times `by`, to channels at .. at + 3 of a row of D. vec: whole groups of 4
+template <typename T>
+__device__ __forceinline__ void store4(T* row, int at, int D, bool vec, const f32x16& a, int x, float by) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    T4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(a[x + e] * by);
+    if (vec) {
+        if (at < D) *reinterpret_cast<T4*>(row + at) = v;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (at + e < D) row[at + e] = v[e];
+    }
+}
+
 // Scores of 32 keys (rows 8 i + 4 half + e) by 32 rows of the problem (columns), as the scores in base 2 with -inf where
 // a pair is left out: s *= c, plus the mask. `gone`: bit k set for key j0 + k that nobody sees (shifted by 4 half).
 // last: the last key that the lane's row sees (causal; INT32_MAX without). mrow: the mask's row (or null).

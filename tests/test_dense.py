@@ -217,9 +217,9 @@ P = 4096  # a stand-in address: these calls end before anything is read
 
 
 def packed(dtype=1, kind=0, causal=0, B=2, Q=5, K=7, H=4, Hk=2, D=8, scale=1.0, q=P, k=P, v=P, mask=0, pad=0, out=P,
-           stats=P):
-    return _dense.ATTN_ARGS.pack(dtype, kind, causal, 0, B, Q, K, H, Hk, D, scale, q, k, v, *([8] * 9), mask, 0, 0, 0,
-                                 pad, out, stats)
+           stats=P, stride=8):
+    return _dense.ATTN_ARGS.pack(dtype, kind, causal, 0, B, Q, K, H, Hk, D, scale, q, k, v, *([8] * 8), stride, mask, 0,
+                                 0, 0, pad, out, stats)
 
 
 @pytest.mark.parametrize('kw,code,message', [
@@ -231,7 +231,7 @@ def packed(dtype=1, kind=0, causal=0, B=2, Q=5, K=7, H=4, Hk=2, D=8, scale=1.0, 
     (dict(scale=0.0), 'TD_E_ARG', 'scale'), (dict(scale=float('nan')), 'TD_E_ARG', 'scale'),
     (dict(kind=3), 'TD_E_ARG', 'mask type'), (dict(kind=1), 'TD_E_ARG', 'null pointer'),
     (dict(q=0), 'TD_E_ARG', 'null pointer'), (dict(v=0), 'TD_E_ARG', 'null pointer'),
-    (dict(out=0), 'TD_E_ARG', 'null pointer'),
+    (dict(out=0), 'TD_E_ARG', 'null pointer'), (dict(stride=-8), 'TD_E_ARG', 'strides'),
 ])
 def test_attention_entries_reject_on_host(lib, kw, code, message):
     a = packed(**kw)
