@@ -5,7 +5,7 @@
  * The conventions of tinydeform.h hold: plain device pointers, int64 sizes, a hipStream_t passed as void*; the library
  * never allocates, frees or synchronises, callers own every buffer (workspaces included), each call may be captured in
  * a HIP graph; TD_OK or a negative TD_E* code is returned, with td_last_error() describing the failure. dtype is TD_F32,
- * TD_F16, TD_BF16 or TD_F64; sums, softmax statistics and norms are float32 (float64 for TD_F64).
+ * TD_F16, TD_BF16 or TD_F64; outputs do not overlap inputs; sums, softmax statistics and norms are float32 (float64 for TD_F64).
  * No counterpart in the reference, whose operator is deformable attention alone.
  */
 #ifndef TINYDEFORM_DENSE_H
