@@ -50,15 +50,17 @@ typedef struct td_attn_args {
     const uint8_t* key_padding; /* [B, K] contiguous, non-zero: no query attends to the key; or NULL */
     void* out;                  /* [B, Q, H * D] contiguous */
     void* stats;                /* [B, H, Q, 2] float32 (float64): the backward's softmax statistics; or NULL */
+    void* out_low;              /* TD_F16, TD_BF16: like out, what rounding took from it, in dtype: the backward's
+                                   grad_out . out then has twice the bits. Or NULL */
 } td_attn_args;
 
-/* Bytes of workspace td_attn_forward needs (0 for many problems), or a negative TD_E* code. No memory is read. */
+/* Bytes of workspace td_attn_forward needs (0 for many problems; a mask takes an eighth of a byte a pair), or a negative TD_E* code. No memory is read. */
 int64_t td_attn_forward_workspace(const td_attn_args* args);
 int td_attn_forward(const td_attn_args* args, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Gradients of td_attn_forward, the probabilities computed again from the scores and `stats`. args: as in the forward
- * call, with the out and stats that it wrote. grad_out [B, Q, H * D], grad_query [B, Q, H, D], grad_key and grad_value
+ * call, with the out, stats and out_low (or NULL) that it wrote. grad_out [B, Q, H * D], grad_query [B, Q, H, D], grad_key and grad_value
  * [B, K, Hk, D] are contiguous, in dtype; grad_query, or grad_key and grad_value together, may be NULL (not computed).
  * No atomics: the results are the same on every run.
  */

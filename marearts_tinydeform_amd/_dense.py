@@ -30,8 +30,8 @@ SIGNATURES = {
     'td_layer_norm_backward': (_int, [_int] + [_vp] * 8 + [_i64, _i64, _vp, _i64, _vp]),
 }
 # td_attn_args: dtype, mask_type, causal, reserved; B, Q, K, H, Hk, D; scale; query, key, value; their strides; mask and
-# its strides; key_padding, out, stats
-ATTN_ARGS = struct.Struct('4i6qd3Q9qQ3q3Q')
+# its strides; key_padding, out, stats, out_low
+ATTN_ARGS = struct.Struct('4i6qd3Q9qQ3q4Q')
 
 
 def _declare(lib):
@@ -119,14 +119,14 @@ def _rows(t):
     return t if t.stride(3) == 1 or t.size(3) == 1 else t.contiguous()
 
 
-def _pack(query, key, value, mask, kind, mask_strides, padding, scale, causal, out, stats):
+def _pack(query, key, value, mask, kind, mask_strides, padding, scale, causal, out, stats, low=None):
     B, Q, H, D = query.shape
     qs, ks, vs = query.stride(), key.stride(), value.stride()
     return ATTN_ARGS.pack(DTYPE_CODES[query.dtype], kind, 1 if causal else 0, 0, B, Q, key.size(1), H, key.size(2), D,
                           scale, query.data_ptr(), key.data_ptr(), value.data_ptr(), qs[0], qs[1], qs[2], ks[0], ks[1],
                           ks[2], vs[0], vs[1], vs[2], 0 if mask is None else mask.data_ptr(), *mask_strides,
                           0 if padding is None else padding.data_ptr(), out.data_ptr(),
-                          0 if stats is None else stats.data_ptr())
+                          0 if stats is None else stats.data_ptr(), 0 if low is None else low.data_ptr())
 
 
 def _workspace(need, device):
@@ -135,47 +135,49 @@ def _workspace(need, device):
     return torch.empty((need,), dtype=torch.uint8, device=device) if need > 0 else None
 
 
-def attn_forward(query, key, value, attn_mask=None, key_padding_mask=None, scale=None, causal=False, want_stats=False):
-    """Attention among tokens (td_attn_forward): out [B, Q, H * D], and with want_stats the softmax statistics
-    [B, H, Q, 2] in float32 (float64 for float64 inputs) that attn_backward takes, else None."""
+def attn_forward(query, key, value, attn_mask=None, key_padding_mask=None, scale=None, causal=False, train=False):
+    """Attention among tokens (td_attn_forward): out [B, Q, H * D], and with train what attn_backward takes: the tensors
+    and the plain values of the call (else None, None)."""
     lib = _require()
     scale, mask, kind, strides, pad = check_attn(query, key, value, attn_mask, key_padding_mask, scale)
     q, k, v = _rows(query), _rows(key), _rows(value)
     B, Q, H, D = q.shape
-    dev = q.device
-    out = torch.empty((B, Q, H * D), dtype=q.dtype, device=dev)
-    stats = torch.empty((B, H, Q, 2), dtype=acc_dtype(q.dtype), device=dev) if want_stats else None
-    if B * Q == 0:
-        return out, stats
-    args = _pack(q, k, v, mask, kind, strides, pad, scale, causal, out, stats)
-    need = lib.td_attn_forward_workspace(args)
-    ws = _workspace(need, dev)
-    _check(lib.td_attn_forward(args, _ptr(ws), need, _stream(dev)))
-    return out, stats
+    dev, dtype = q.device, q.dtype
+    out = torch.empty((B, Q, H * D), dtype=dtype, device=dev)
+    stats = low = None
+    if train:
+        stats = torch.empty((B, H, Q, 2), dtype=acc_dtype(dtype), device=dev)
+        if dtype in (torch.float16, torch.bfloat16):  # what rounding took from out: grad_out . out needs it
+            low = torch.empty((B, Q, H * D), dtype=dtype, device=dev)
+    if B * Q > 0:
+        args = _pack(q, k, v, mask, kind, strides, pad, scale, causal, out, stats, low)
+        need = lib.td_attn_forward_workspace(args)
+        ws = _workspace(need, dev)
+        _check(lib.td_attn_forward(args, _ptr(ws), need, _stream(dev)))
+    if not train:
+        return out, None, None
+    return out, (q, k, v, mask, pad, out, stats, low), (kind, strides, scale, causal)
 
 
-def attn_backward(query, key, value, attn_mask, key_padding_mask, scale, causal, out, stats, grad_out, need_query=True,
-                  need_key_value=True):
-    """Gradients of attn_forward (td_attn_backward) from its out and stats: grad_query like query, grad_key and
+def attn_backward(tensors, values, grad_out, need_query=True, need_key_value=True):
+    """Gradients of attn_forward (td_attn_backward) from what it gave for training: grad_query like query, grad_key and
     grad_value like key; None for those not needed."""
     lib = _require()
-    scale, mask, kind, strides, pad = check_attn(query, key, value, attn_mask, key_padding_mask, scale)
-    q, k, v = _rows(query), _rows(key), _rows(value)
-    B, Q, H, D = q.shape
+    q, k, v, mask, pad, out, stats, low = tensors
+    kind, strides, scale, causal = values
     if grad_out.shape != out.shape or grad_out.dtype != q.dtype or grad_out.device != q.device:
         raise RuntimeError('grad_out must be [B, Q, H * D] like the forward output')
-    if stats.shape != (B, H, Q, 2) or out.shape != (B, Q, H * D):
-        raise RuntimeError('out and stats must be those of the forward')
-    dev, go = q.device, grad_out.contiguous()
-    dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if need_query else None
-    dk = torch.empty(k.shape, dtype=k.dtype, device=dev) if need_key_value else None
-    dv = torch.empty(v.shape, dtype=v.dtype, device=dev) if need_key_value else None
-    if B == 0 or (Q == 0 and k.size(1) == 0):
-        return dq, dk, dv
-    args = _pack(q, k, v, mask, kind, strides, pad, scale, causal, out, stats)
-    need = lib.td_attn_backward_workspace(args)
-    ws = _workspace(need, dev)
-    _check(lib.td_attn_backward(args, go.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), need, _stream(dev)))
+    dev, dtype, go = q.device, q.dtype, grad_out.contiguous()
+    dq = torch.empty(q.shape, dtype=dtype, device=dev) if need_query else None
+    dk = dv = None
+    if need_key_value:
+        dk = torch.empty(k.shape, dtype=dtype, device=dev)
+        dv = torch.empty(k.shape, dtype=dtype, device=dev)
+    if q.size(0) * (q.size(1) + k.size(1)) > 0:
+        args = _pack(q, k, v, mask, kind, strides, pad, scale, causal, out, stats, low)
+        need = lib.td_attn_backward_workspace(args)
+        ws = _workspace(need, dev)
+        _check(lib.td_attn_backward(args, go.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), need, _stream(dev)))
     return dq, dk, dv
 
 
@@ -211,9 +213,9 @@ def _contiguous(t):
     return None if t is None else t.contiguous()
 
 
-def layer_norm_forward(x, weight, bias, residual=None, eps=1e-5, want_stats=False):
-    """Layer norm of x (+ residual) (td_layer_norm_forward): out like x, and with want_stats mean and rstd of each row
-    [rows, 2] in float32 (float64), else None."""
+def layer_norm_forward(x, weight, bias, residual=None, eps=1e-5, train=False):
+    """Layer norm of x (+ residual) (td_layer_norm_forward): out like x, and with train the tensors that
+    layer_norm_backward takes (else None)."""
     lib = _require()
     rows, C = check_norm(x, weight, bias, residual)
     if not (eps >= 0 and math.isfinite(eps)):
@@ -221,27 +223,26 @@ def layer_norm_forward(x, weight, bias, residual=None, eps=1e-5, want_stats=Fals
     dev = x.device
     x, weight, bias, residual = x.contiguous(), _contiguous(weight), _contiguous(bias), _contiguous(residual)
     out = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    stats = torch.empty((rows, 2), dtype=acc_dtype(x.dtype), device=dev) if want_stats else None
+    stats = torch.empty((rows, 2), dtype=acc_dtype(x.dtype), device=dev) if train else None
     if rows > 0:
         _check(lib.td_layer_norm_forward(DTYPE_CODES[x.dtype], x.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias),
                                          out.data_ptr(), _ptr(stats), rows, C, eps, _stream(dev)))
-    return out, stats
+    return out, (x, weight, residual, stats) if train else None
 
 
-def layer_norm_backward(x, weight, residual, stats, grad_out, need_weight=True, need_bias=True):
-    """Gradients of layer_norm_forward (td_layer_norm_backward): grad_x like x (the residual's too), grad_weight and
-    grad_bias [C], None where not needed."""
+def layer_norm_backward(tensors, grad_out, need_weight=True, need_bias=True):
+    """Gradients of layer_norm_forward (td_layer_norm_backward) from what it gave for training: grad_x like x (the
+    residual's too), grad_weight and grad_bias [C], None where not needed."""
     lib = _require()
-    rows, C = check_norm(x, weight, None, residual)
+    x, weight, residual, stats = tensors
     if grad_out.shape != x.shape or grad_out.dtype != x.dtype or grad_out.device != x.device:
         raise RuntimeError('grad_out must be like the forward output')
-    if stats.shape != (rows, 2):
-        raise RuntimeError('stats must be those of the forward')
-    dev, code = x.device, DTYPE_CODES[x.dtype]
-    x, weight, residual, go = x.contiguous(), _contiguous(weight), _contiguous(residual), grad_out.contiguous()
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    dw = torch.empty((C,), dtype=x.dtype, device=dev) if need_weight else None
-    db = torch.empty((C,), dtype=x.dtype, device=dev) if need_bias else None
+    rows, C = stats.size(0), x.size(-1)
+    dev, dtype, go = x.device, x.dtype, grad_out.contiguous()
+    code = DTYPE_CODES[dtype]
+    dx = torch.empty(x.shape, dtype=dtype, device=dev)
+    dw = torch.empty((C,), dtype=dtype, device=dev) if need_weight else None
+    db = torch.empty((C,), dtype=dtype, device=dev) if need_bias else None
     need = lib.td_layer_norm_backward_workspace(code, rows, C) if need_weight or need_bias else 0
     ws = _workspace(need, dev)
     _check(lib.td_layer_norm_backward(code, x.data_ptr(), _ptr(residual), _ptr(weight), stats.data_ptr(), go.data_ptr(),

@@ -23,6 +23,13 @@ struct AttnParams {
     int64_t diag;   // K - Q: with causal, query i sees the keys j <= i + diag
     double scale;
     float c;        // scale * log2(e): scores in base 2
+    void* out_low;  // 16-bit types: out's rounding errors, or null
+    // a mask as bits (attn_mask_kernel): row b * bs[0] + h * bs[1] + i * bs[2] has words of 32 keys, set for pairs left
+    // out; kinds[(that row's 32-row tile)][word]: MaskKind of the 32 x 32 pairs
+    uint32_t* bits;
+    uint8_t* kinds;
+    int64_t bs[3], kinds_bs[2];  // rows; tiles (kinds_bs: batch, head), 0 where shared
+    int words;                   // of a row
     // backward
     const void* go;
     void *dq, *dk, *dv;
@@ -31,7 +38,12 @@ struct AttnParams {
     void* ws;
 };
 
+enum MaskKind { kMaskNone = 0, kMaskBits = 1, kMaskValues = 2, kMaskAll = 3 };
+
 AttnParams attn_params(const td_attn_args& a);
+// The mask as bits, at `at` (16-byte aligned); returns the bytes they take, a multiple of 16. With at null only that.
+int64_t plan_mask(AttnParams& p, void* at);
+int launch_mask(int dtype, const AttnParams& p, hipStream_t stream);
 
 // On the matrix units, for float32, float16 and bfloat16 (td_attn_forward.hip)
 int64_t attn_forward_workspace(int dtype, const AttnParams& p);

@@ -257,6 +257,105 @@ int launch_attn_backward_generic(int dtype, const AttnParams& p, hipStream_t str
     }
 }
 
+namespace {
+
+// The mask as bits, a wavefront for 32 rows by two words of 32 keys: each mask entry is read once here instead of once by
+// every head that shares it, and a tile that the mask leaves as it is, or leaves nothing of, costs its readers nothing.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_mask_kernel(AttnParams p, int64_t tiles, int tile_rows, int mask_rows,
+                                                        int mask_heads) {
+    const int lane = threadIdx.x % kWave, half = lane >> 5, pairs = (p.words + 1) / 2;
+    const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
+    if (id >= tiles * pairs) return;
+    const int word = static_cast<int>(id % pairs) * 2 + half, j0 = word * 32;
+    const int64_t tile = id / pairs, at = tile / tile_rows;  // at: batch and head of the mask
+    const int row = static_cast<int>(tile % tile_rows) * 32 + (lane & 31);
+    const int64_t b = at / mask_heads, h = at % mask_heads;
+    uint32_t bits = ~0u;
+    bool values = false;
+    const bool in = row < mask_rows && word < p.words;
+    if (in) {
+        const int64_t m0 = b * p.ms[0] + h * p.ms[1] + row * p.ms[2] + j0;
+        const int left = p.K - j0;
+        if (p.mask_type == TD_MASK_BYTES) {
+            const uint8_t* m = static_cast<const uint8_t*>(p.mask) + m0;
+            if (left >= 32) {
+                uint32_t v[8];
+                __builtin_memcpy(v, m, 32);
+                bits = 0;
+#pragma unroll
+                for (int k = 0; k < 32; ++k) bits |= ((v[k / 4] >> (8 * (k % 4))) & 0xffu ? 1u : 0u) << k;
+            } else {
+                for (int k = 0; k < left; ++k)
+                    if (m[k] == 0) bits &= ~(1u << k);
+            }
+        } else {
+            const T* m = static_cast<const T*>(p.mask) + m0;
+            for (int k = 0; k < 32 && k < left; ++k) {
+                const float v = static_cast<float>(m[k]);
+                if (v != neg_inf<float>()) bits &= ~(1u << k);
+                values |= v != 0.f && v != neg_inf<float>();
+            }
+        }
+        p.bits[(at * mask_rows + row) * p.words + word] = bits;
+    }
+    // keys past the end are set in the bits; rows past the end say nothing
+    const uint32_t past = p.K - j0 >= 32 || word >= p.words ? 0u : ~0u << (p.K - j0);
+    const uint64_t mine = half ? ~uint64_t{0} << 32 : ~uint64_t{0} >> 32;
+    const uint64_t any_values = __ballot(in && values) & mine, any_bits = __ballot(in && (bits & ~past)) & mine;
+    const uint64_t any_left = __ballot(in && bits != ~0u) & mine;
+    if ((lane & 31) == 0 && word < p.words)
+        p.kinds[tile * p.words + word] = static_cast<uint8_t>(any_left == 0     ? kMaskAll
+                                                              : any_values != 0 ? kMaskValues
+                                                              : any_bits != 0 || past != 0 ? kMaskBits
+                                                                                           : kMaskNone);
+}
+
+struct MaskShape {
+    int batches, heads, rows, tile_rows;
+};
+MaskShape mask_shape(const AttnParams& p) {
+    MaskShape m{p.ms[0] == 0 ? 1 : p.B, p.ms[1] == 0 ? 1 : p.H, p.ms[2] == 0 ? 1 : p.Q, 0};
+    m.tile_rows = (m.rows + 31) / 32;
+    return m;
+}
+
+}  // namespace
+
+int64_t plan_mask(AttnParams& p, void* at) {
+    if (p.mask_type == TD_MASK_NONE || p.K == 0 || p.Q == 0) return 0;
+    const MaskShape m = mask_shape(p);
+    p.words = (p.K + 31) / 32;
+    const int64_t heads = static_cast<int64_t>(m.batches) * m.heads;
+    const int64_t bits = (heads * m.rows * p.words * 4 + 15) / 16 * 16;
+    const int64_t kinds = (heads * m.tile_rows * p.words + 15) / 16 * 16;
+    p.bits = static_cast<uint32_t*>(at);
+    p.kinds = static_cast<uint8_t*>(at) + bits;
+    const int64_t per_batch = m.heads;
+    p.bs[0] = m.batches == 1 ? 0 : per_batch * m.rows;
+    p.bs[1] = m.heads == 1 ? 0 : m.rows;
+    p.bs[2] = m.rows == 1 ? 0 : 1;
+    p.kinds_bs[0] = m.batches == 1 ? 0 : per_batch * m.tile_rows;
+    p.kinds_bs[1] = m.heads == 1 ? 0 : m.tile_rows;
+    return bits + kinds;
+}
+
+int launch_mask(int dtype, const AttnParams& p, hipStream_t stream) {
+    if (p.words == 0) return 0;
+    const MaskShape m = mask_shape(p);
+    const int64_t tiles = static_cast<int64_t>(m.batches) * m.heads * m.tile_rows;
+    const int64_t groups = (tiles * ((p.words + 1) / 2) + 3) / 4;
+    if (groups > 16777215) return set_error(TD_E_ARG, "attention: the mask has too many entries");
+    const dim3 grid(static_cast<unsigned>(groups));
+    if (dtype == kF32)
+        hipLaunchKernelGGL((attn_mask_kernel<float>), grid, dim3(256), 0, stream, p, tiles, m.tile_rows, m.rows, m.heads);
+    else if (dtype == kF16)
+        hipLaunchKernelGGL((attn_mask_kernel<f16>), grid, dim3(256), 0, stream, p, tiles, m.tile_rows, m.rows, m.heads);
+    else
+        hipLaunchKernelGGL((attn_mask_kernel<bf16>), grid, dim3(256), 0, stream, p, tiles, m.tile_rows, m.rows, m.heads);
+    return launched("attention mask");
+}
+
 AttnParams attn_params(const td_attn_args& a) {
     AttnParams p{};
     p.q = a.query;
@@ -266,6 +365,7 @@ AttnParams attn_params(const td_attn_args& a) {
     p.pad = a.key_padding;
     p.out = a.out;
     p.stats = a.stats;
+    p.out_low = a.dtype == TD_F16 || a.dtype == TD_BF16 ? a.out_low : nullptr;
     for (int i = 0; i < 3; ++i) {
         p.qs[i] = a.query_stride[i];
         p.ks[i] = a.key_stride[i];

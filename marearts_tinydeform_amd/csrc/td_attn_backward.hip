@@ -52,11 +52,18 @@ __global__ __launch_bounds__(256) void attn_info_kernel(AttnParams p, RowInfo in
             const int i = static_cast<int>(fast_div(p.gdiv, n)), h = hk * p.G + n - i * p.G;
             const int64_t at = ((static_cast<int64_t>(b) * p.Q + i) * p.H + h) * p.D;
             const T *g = static_cast<const T*>(p.go) + at, *o = static_cast<const T*>(p.out) + at;
+            const T* low = p.out_low == nullptr ? nullptr : static_cast<const T*>(p.out_low) + at;
             if (vec) {
                 for (int d = part * E; d < p.D; d += 4 * E) {
                     float x[E], y[E];
                     VecIO<T, E>::unpack(VecIO<T, E>::load(g + d), x);
                     VecIO<T, E>::unpack(VecIO<T, E>::load(o + d), y);
+                    if (low != nullptr) {
+                        float z[E];
+                        VecIO<T, E>::unpack(VecIO<T, E>::load(low + d), z);
+#pragma unroll
+                        for (int e = 0; e < E; ++e) y[e] += z[e];
+                    }
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
                         delta = fmaf(x[e], y[e], delta);
@@ -65,7 +72,8 @@ __global__ __launch_bounds__(256) void attn_info_kernel(AttnParams p, RowInfo in
                 }
             } else {
                 for (int d = part; d < p.D; d += 4) {
-                    delta = fmaf(static_cast<float>(g[d]), static_cast<float>(o[d]), delta);
+                    const float y = static_cast<float>(o[d]) + (low == nullptr ? 0.f : static_cast<float>(low[d]));
+                    delta = fmaf(static_cast<float>(g[d]), y, delta);
                     see(static_cast<float>(g[d]));
                 }
             }
@@ -124,14 +132,15 @@ template <typename T, int DP, bool WK>
 constexpr int dq_key_tile() {
     return WK || DP * static_cast<int>(sizeof(T)) > 128 ? 32 : 64;
 }
-template <typename T, int DP, bool SLOW>
+// Wavefronts a SIMD that the registers leave room for without spills
+template <typename T, int DP, bool WK, bool SLOW>
 constexpr int dq_min_waves() {
     constexpr int bytes = DP * static_cast<int>(sizeof(T));
-    return bytes <= 64 ? (SLOW ? 2 : 3) : bytes <= 128 ? 2 : 1;
+    return bytes <= 64 ? (SLOW ? 2 : 3) : bytes <= 128 || (bytes <= 256 && !WK) ? 2 : 1;
 }
 
 template <typename T, int DP, bool WK, bool MASK, bool VEC>
-__global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dq_kernel(AttnParams p, RowInfo info,
+__global__ __launch_bounds__(256, (dq_min_waves<T, DP, WK, MASK>())) void attn_dq_kernel(AttnParams p, RowInfo info,
                                                                                     bool vec_out, int tiles) {
     using R = TileRows<T, DP>;
     constexpr int KT = dq_key_tile<T, DP, WK>(), NT = WK ? 64 : 256, ND = DP / 32;
@@ -165,10 +174,7 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dq_ke
     const f32x4 ri = info.rows[static_cast<int64_t>(bh) * p.rows + (live ? r : 0)];
     const float ds_scale = ds_factor<T>(p, info, bh, lane);
     const float delta = ri[2] * ds_scale;
-    const unsigned char* const mrow =
-        !MASK ? nullptr
-              : static_cast<const unsigned char*>(p.mask) + (b * p.ms[0] + h * p.ms[1] + i * p.ms[2]) *
-                                                                (p.mask_type == TD_MASK_FLOAT ? sizeof(T) : 1);
+    const T* const mrow = MASK ? static_cast<const T*>(p.mask) + b * p.ms[0] + h * p.ms[1] + i * p.ms[2] : nullptr;
     // an additive mask may make m so large that log2 l is lost beside it: it is subtracted after t - m then
     const bool apart = MASK && p.mask_type == TD_MASK_FLOAT;
     const float from = apart ? ri[0] : ri[0] + ri[1] - kPShift<T>, then = apart ? ri[1] - kPShift<T> : 0.f;
@@ -205,7 +211,11 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dq_ke
     constexpr uint64_t all = KT == 64 ? ~uint64_t{0} : (uint64_t{1} << (KT & 63)) - 1;
     int64_t j0 = WK ? wave * KT : 0;
     uint64_t gone = __ballot(pad_byte(j0)), gone_next;
+    MaskWord mw[KT / 32] = {};
     auto fetch = [&](int64_t at, uint64_t g) {
+        if constexpr (MASK)
+#pragma unroll
+            for (int x = 0; x < KT / 32; ++x) mw[x] = mask_word(p, b, h, i, static_cast<int>(at / 32) + x);
         ks.load(kb + at * p.ks[1], k_row, g & all, p.D, t);
         vs.load(vb + at * p.vs[1], v_row, g & all, p.D, t);
     };
@@ -220,16 +230,31 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dq_ke
         else
             __syncthreads();
         gone_next = __ballot(next_pad);
+        uint32_t bits[KT / 32];
+        bool masked[KT / 32], values[KT / 32], none[KT / 32];
+#pragma unroll
+        for (int x = 0; x < KT / 32; ++x) {
+            const uint32_t pad_bits = static_cast<uint32_t>(gone >> (32 * x));
+            const int jx = static_cast<int>(j0) + 32 * x;
+            bits[x] = mw[x].bits;
+            masked[x] = pad_bits != 0 || jx + 31 > seen_all;
+            none[x] = pad_bits == ~0u || jx > seen_any;
+            values[x] = false;
+            if constexpr (MASK) {
+                masked[x] |= __any(mw[x].kind != kMaskNone);
+                values[x] = __any(mw[x].kind == kMaskValues);
+                none[x] |= __all(mw[x].kind == kMaskAll);
+            }
+        }
         if (j0 + step < kend) {
             fetch(j0 + step, gone_next);
             next_pad = pad_byte(j0 + 2 * step);
         }
         const int j = static_cast<int>(j0);
-        if ((gone & all) != all && j <= seen_any) {
-            const bool whole = j + KT <= p.K;
-            const bool masked = (gone & all) != 0 || mrow != nullptr || j + KT - 1 > seen_all;
+        {
 #pragma unroll
             for (int x = 0; x < KT / 32; ++x) {
+                if (none[x]) continue;
                 f32x16 s = f32x16{0.f}, dp = f32x16{0.f};
 #pragma unroll
                 for (int c = 0; c < R::kChunks; ++c) {
@@ -237,10 +262,11 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dq_ke
                     dp = Mma<T>::mul(R::rows(vt_lds, 32 * x, c, lane), gf[c], dp);
                 }
                 float cc = p.c;
-                if (masked) {
+                if (masked[x]) {
                     cc = 1.f;
-                    mask_scores<T>(s, p, j + 32 * x, static_cast<unsigned>(gone >> (32 * x + 4 * half)), last, mrow, half,
-                                   whole);
+                    mask_scores<T>(s, p.c,
+                                   bits[x] | static_cast<uint32_t>(gone >> (32 * x)) | beyond(j + 32 * x, last),
+                                   values[x] ? mrow + j + 32 * x : nullptr, p.K - j - 32 * x, half);
                 }
                 f32x16 ds;
 #pragma unroll
@@ -305,13 +331,25 @@ constexpr int dkv_row_tile() {
     return WK || DP * static_cast<int>(sizeof(T)) > 128 ? 32 : 64;
 }
 
+// What LDS holds of a row beside its elements: m, log2 l, delta, the mask words of the workgroup's keys, and with a mask
+// its kind for each word and the row's offset in it
+template <typename T, int DP, bool WK>
+constexpr bool v_in_lds() {
+    return !WK && DP * static_cast<int>(sizeof(T)) == 256;
+}
+template <bool WK, bool MASK>
+constexpr int dkv_row_bytes() {
+    return 12 + (WK ? 4 : 16) + (MASK ? 8 + (WK ? 4 : 16) : 0) + (WK ? 0 : 4);  // a multiple of 8
+}
+
 template <typename T, int DP, bool WK, bool MASK, bool VEC>
-__global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dkv_kernel(AttnParams p, RowInfo info,
+__global__ __launch_bounds__(256, (dq_min_waves<T, DP, WK, MASK>())) void attn_dkv_kernel(AttnParams p, RowInfo info,
                                                                                      bool vec_out, int tiles) {
     using R = TileRows<T, DP>;
     constexpr int RT = dkv_row_tile<T, DP, WK>(), NT = WK ? 64 : 256, ND = DP / 32;
     constexpr int kTile = RT * R::kPitch;
-    constexpr int kArea = 2 * kTile + RT * 24;  // two tiles, m and delta (or m, log2 l, delta) and mask offsets of the rows
+    constexpr int KW = WK ? 1 : 4;  // words of 32 keys that the workgroup's keys have
+    constexpr int kArea = 2 * kTile + RT * dkv_row_bytes<WK, MASK>();
     extern __shared__ __align__(16) unsigned char lds[];
     const int id = xcd_order(static_cast<int>(blockIdx.x), p.B * p.Hk * tiles);
     if (id < 0) return;
@@ -325,19 +363,27 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dkv_k
     float* const m_lds = reinterpret_cast<float*>(g_lds + kTile);
     float* const l_lds = m_lds + RT;
     float* const d_lds = l_lds + RT;
-    int64_t* const o_lds = reinterpret_cast<int64_t*>(d_lds + RT);  // 12 RT bytes on: a multiple of 8
+    uint32_t* const w_lds = reinterpret_cast<uint32_t*>(d_lds + RT);   // [KW][RT]
+    int* const k_lds = reinterpret_cast<int*>(w_lds + KW * RT);        // [KW][RT], with a mask
+    int64_t* const o_lds = reinterpret_cast<int64_t*>(k_lds + KW * RT);
 
     // the lane's key
     const int key0 = tile * (WK ? 32 : 128), wkey0 = key0 + (WK ? 0 : wave * 32), j = wkey0 + (lane & 31);
     const bool live = j < p.K && (p.pad == nullptr || p.pad[static_cast<int64_t>(b) * p.K + j] == 0);
-    u32x4 kf[R::kChunks], vf[R::kChunks];
+    constexpr bool kVInLds = v_in_lds<T, DP, WK>();
+    u32x4 kf[R::kChunks], vf[kVInLds ? 1 : R::kChunks];
+    unsigned char* const v_own = lds + kArea;
     {
         const T* k = static_cast<const T*>(p.k) + b * p.ks[0] + j * p.ks[1] + hk * p.ks[2];
         const T* v = static_cast<const T*>(p.v) + b * p.vs[0] + j * p.vs[1] + hk * p.vs[2];
 #pragma unroll
         for (int c = 0; c < R::kChunks; ++c) {
             kf[c] = live ? row_piece<T, VEC>(k, c * 32 + half * 16, p.D) : u32x4{0u, 0u, 0u, 0u};
-            vf[c] = live ? row_piece<T, VEC>(v, c * 32 + half * 16, p.D) : u32x4{0u, 0u, 0u, 0u};
+            const u32x4 vc = live ? row_piece<T, VEC>(v, c * 32 + half * 16, p.D) : u32x4{0u, 0u, 0u, 0u};
+            if constexpr (kVInLds)  // the wavefront's own rows: read back by this wavefront alone
+                *reinterpret_cast<u32x4*>(v_own + (wave * 32 + (lane & 31)) * R::kPitch + c * 32 + half * 16) = vc;
+            else
+                vf[c] = vc;
         }
     }
     const float ds_scale = ds_factor<T>(p, info, bh, lane);
@@ -384,6 +430,9 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dkv_k
     }
     f32x4 ri = f32x4{0.f, 0.f, 0.f, 0.f};
     int64_t mo = 0;
+    uint32_t words[KW] = {};
+    int kinds[KW] = {};
+    const bool bits = MASK || p.causal;
     auto fetch = [&](int64_t at) {
         from_row = at;
         const int64_t left = p.rows - at;
@@ -398,10 +447,17 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dkv_k
         if (t < RT) {
             const bool in = t < left;
             ri = in ? ib[at + t] : f32x4{__builtin_inff(), 0.f, 0.f, 0.f};
-            if (MASK) {
+            if (bits) {
                 const int i = static_cast<int>(fast_div(p.gdiv, static_cast<uint32_t>(in ? at + t : 0)));
-                const int g = static_cast<int>(in ? at + t : 0) - i * p.G;
-                mo = b * p.ms[0] + (hk * p.G + g) * p.ms[1] + i * p.ms[2];
+                const int h = hk * p.G + static_cast<int>(in ? at + t : 0) - i * p.G;
+                if (MASK) mo = b * p.ms[0] + h * p.ms[1] + i * p.ms[2];
+#pragma unroll
+                for (int w = 0; w < KW; ++w) {
+                    MaskWord m{0u, kMaskNone};
+                    if (MASK) m = mask_word(p, b, h, i, key0 / 32 + w);
+                    words[w] = m.bits | (p.causal ? beyond(key0 + 32 * w, i + diag) : 0u);
+                    kinds[w] = in ? m.kind : kMaskAll;
+                }
             }
         }
     };
@@ -421,6 +477,13 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dkv_k
             l_lds[t] = ri[1] - kPShift<T>;
             d_lds[t] = ri[2] * ds_scale;
             if (MASK) o_lds[t] = mo;
+            if (bits) {
+#pragma unroll
+                for (int w = 0; w < KW; ++w) {
+                    w_lds[w * RT + t] = words[w];
+                    if (MASK) k_lds[w * RT + t] = kinds[w];
+                }
+            }
         }
         if (WK)
             wave_sync();
@@ -428,32 +491,44 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dkv_k
             __syncthreads();
         if (r0 + step < p.rows) fetch(r0 + step);
         if (any && r0 + RT > wfirst_row) {
-            const bool masked = MASK || r0 < whole_row;
+            const uint32_t* const my_words = w_lds + (WK ? 0 : wave * RT);
 #pragma unroll
             for (int x = 0; x < RT / 32; ++x) {
+                bool masked = r0 + 32 * x < whole_row, values = false;
+                if constexpr (MASK) {
+                    const int kind = k_lds[(WK ? 0 : wave * RT) + 32 * x + (lane & 31)];
+                    if (__all(kind == kMaskAll)) continue;
+                    masked |= __any(kind != kMaskNone);
+                    values = __any(kind == kMaskValues);
+                }
                 f32x16 s = f32x16{0.f}, dp = f32x16{0.f};
 #pragma unroll
                 for (int c = 0; c < R::kChunks; ++c) {
                     s = Mma<T>::mul(R::rows(q_lds, 32 * x, c, lane), kf[c], s);
-                    dp = Mma<T>::mul(R::rows(g_lds, 32 * x, c, lane), vf[c], dp);
+                    dp = Mma<T>::mul(R::rows(g_lds, 32 * x, c, lane),
+                                     kVInLds ? R::rows(v_own, wave * 32, c, lane) : vf[kVInLds ? 0 : c], dp);
                 }
                 float cc = p.c;
                 if (masked) {
                     cc = 1.f;
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int row = 32 * x + 8 * (e >> 2) + 4 * half + (e & 3);
-                        bool out = false;
-                        float add = 0.f;
-                        if (MASK && p.mask_type == TD_MASK_FLOAT) {
-                            add = mask_log2(static_cast<float>(static_cast<const T*>(p.mask)[o_lds[row] + mask_key]));
-                            out = add == kNegInf;
-                        } else if (MASK && p.mask_type == TD_MASK_BYTES) {
-                            out = static_cast<const uint8_t*>(p.mask)[o_lds[row] + mask_key] != 0;
+                    for (int y = 0; y < 4; ++y) {
+                        const int row = 32 * x + 8 * y + 4 * half;
+                        const u32x4 w4 = *reinterpret_cast<const u32x4*>(my_words + row);
+                        float add[4] = {0.f, 0.f, 0.f, 0.f};
+                        if (MASK && values) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                add[e] = mask_log2(
+                                    static_cast<float>(static_cast<const T*>(p.mask)[o_lds[row + e] + mask_key]));
+                            __builtin_amdgcn_sched_barrier(0);  // four loads at a time: registers
                         }
-                        if (p.causal)
-                            out |= j > static_cast<int>(fast_div(p.gdiv, static_cast<uint32_t>(r0 + row))) + diag;
-                        s[e] = out ? kNegInf : fmaf(s[e], p.c, add);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const unsigned w = w4[e];
+                            const float t = fmaf(s[4 * y + e], p.c, add[e]);
+                            s[4 * y + e] = (w >> (lane & 31)) & 1u ? kNegInf : t;
+                        }
                     }
                 }
                 f32x16 ds;
@@ -579,9 +654,10 @@ int run_dq(const AttnParams& p, const BackShape& s, const RowInfo& info, hipStre
 template <typename T, int DP, bool WK, bool MASK, bool VEC>
 int run_dkv(const AttnParams& p, const BackShape& s, const RowInfo& info, hipStream_t stream) {
     static std::atomic<uint64_t> done{0};
-    constexpr int RT = dkv_row_tile<T, DP, WK>(), area = 2 * RT * TileRows<T, DP>::kPitch + RT * 24;
+    constexpr int RT = dkv_row_tile<T, DP, WK>(), area = 2 * RT * TileRows<T, DP>::kPitch + RT * dkv_row_bytes<WK, MASK>();
     constexpr int join = 2 * 32 * (DP + 4) * 4;
-    constexpr int bytes = WK ? (4 * area > join ? 4 * area : join) : area;
+    constexpr int own = v_in_lds<T, DP, WK>() ? 128 * TileRows<T, DP>::kPitch : 0;
+    constexpr int bytes = WK ? (4 * area > join ? 4 * area : join) : area + own;
     static_assert(bytes <= 160 * 1024, "LDS of a CU");
     auto* const fn = &attn_dkv_kernel<T, DP, WK, MASK, VEC>;
     const hipError_t e =
@@ -623,9 +699,9 @@ int run_dp(const AttnParams& p, const BackShape& s, const RowInfo& info, hipStre
     return rc;
 }
 
-RowInfo info_of(const AttnParams& p) {
+RowInfo info_of(const AttnParams& p, void* at) {
     RowInfo r{};
-    r.rows = static_cast<f32x4*>(p.ws);
+    r.rows = static_cast<f32x4*>(at);
     r.amax = reinterpret_cast<float*>(r.rows + static_cast<int64_t>(p.B) * p.Hk * p.rows);
     r.blocks = (p.rows + kInfoRows - 1) / kInfoRows;
     r.key_blocks = (p.K + kInfoRows - 1) / kInfoRows;
@@ -635,16 +711,18 @@ RowInfo info_of(const AttnParams& p) {
 }  // namespace
 
 template <typename T>
-int launch_attn_backward_t(int dtype, const AttnParams& p, hipStream_t stream) {
+int launch_attn_backward_t(int dtype, const AttnParams& given, hipStream_t stream) {
+    AttnParams p = given;
     const BackShape s = back_shape(dtype, p);
-    const RowInfo info = info_of(p);
+    const RowInfo info = info_of(p, static_cast<unsigned char*>(p.ws) + plan_mask(p, p.ws));
+    int rc = launch_mask(dtype, p, stream);
+    if (rc != 0) return rc;
     const int64_t blocks =
         static_cast<int64_t>(p.B) * p.Hk * (info.blocks + (kScaled<T> ? info.key_blocks : 0));
     const bool vec = p.D * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(p.go) % 16 == 0 &&
-                     reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
+                     (reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.out_low)) % 16 == 0;
     if (blocks > 0)
         hipLaunchKernelGGL((attn_info_kernel<T>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, p, info, vec);
-    int rc;
     switch (padded_width(p.D)) {
         case 32: rc = run_dp<T, 32>(p, s, info, stream); break;
         case 64: rc = run_dp<T, 64>(p, s, info, stream); break;
@@ -662,8 +740,9 @@ template int launch_attn_backward_t<float>(int, const AttnParams&, hipStream_t);
 int64_t attn_backward_workspace(int dtype, const AttnParams& p) {
     const int64_t rows = static_cast<int64_t>(p.B) * p.H * p.Q;
     if (dtype == kF64) return rows * 8;
-    const RowInfo r = info_of(p);
-    return rows * 16 + (dtype == kF16 ? static_cast<int64_t>(p.B) * p.Hk * (r.blocks + r.key_blocks) * 4 : 0);
+    const RowInfo r = info_of(p, nullptr);
+    AttnParams q = p;
+    return plan_mask(q, nullptr) + rows * 16 + (dtype == kF16 ? static_cast<int64_t>(p.B) * p.Hk * (r.blocks + r.key_blocks) * 4 : 0);
 }
 
 int launch_attn_backward(int dtype, const AttnParams& p, hipStream_t stream) {

@@ -75,11 +75,7 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
         for (int c = 0; c < R::kChunks; ++c)
             qf[c] = live ? row_piece<T, VEC>(q, c * 32 + half * 16, p.D) : u32x4{0u, 0u, 0u, 0u};
     }
-    const unsigned char* const mrow =
-        !MASK
-            ? nullptr
-            : static_cast<const unsigned char*>(p.mask) + (b * p.ms[0] + h * p.ms[1] + i * p.ms[2]) *
-                                                              (p.mask_type == TD_MASK_FLOAT ? sizeof(T) : 1);
+    const T* const mrow = MASK ? static_cast<const T*>(p.mask) + b * p.ms[0] + h * p.ms[1] + i * p.ms[2] : nullptr;
     const int diag = static_cast<int>(p.diag);
     const int last = p.causal ? i + diag : 2147483647;
 
@@ -122,7 +118,11 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
     constexpr uint64_t all = KT == 64 ? ~uint64_t{0} : (uint64_t{1} << (KT & 63)) - 1;
     int64_t j0 = k0 + (WK ? wave * KT : 0);
     uint64_t gone = __ballot(pad_byte(j0)), gone_next;
+    MaskWord mw[KT / 32] = {};
     auto fetch = [&](int64_t at, uint64_t g) {
+        if constexpr (MASK)
+#pragma unroll
+            for (int x = 0; x < KT / 32; ++x) mw[x] = mask_word(p, b, h, i, static_cast<int>(at / 32) + x);
         ks.load(kb + at * p.ks[1], k_row, g & all, p.D, t);
         vs.load(vb + at * p.vs[1], v_row, g & all, p.D, t);
     };
@@ -137,14 +137,24 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
         else
             __syncthreads();
         gone_next = __ballot(next_pad);
+        // what the tile's scores have to be masked by
+        bool masked = (gone & all) != 0 || static_cast<int>(j0) + KT - 1 > seen_all, values = false, none = MASK;
+        uint32_t bits[KT / 32];
+#pragma unroll
+        for (int x = 0; x < KT / 32; ++x) {
+            bits[x] = mw[x].bits;
+            if constexpr (MASK) {
+                masked |= __any(mw[x].kind != kMaskNone);
+                values |= __any(mw[x].kind == kMaskValues);
+                none &= __all(mw[x].kind == kMaskAll);
+            }
+        }
         if (j0 + step < kend) {
             fetch(j0 + step, gone_next);
             next_pad = pad_byte(j0 + 2 * step);
         }
         const int j = static_cast<int>(j0);
-        if ((gone & all) != all && j <= seen_any) {
-            const bool whole = j + KT <= p.K;
-            const bool masked = (gone & all) != 0 || mrow != nullptr || j + KT - 1 > seen_all;
+        if ((gone & all) != all && j <= seen_any && !none) {
             f32x16 s[KT / 32];
 #pragma unroll
             for (int x = 0; x < KT / 32; ++x) {
@@ -158,8 +168,9 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
                 cc = 1.f;
 #pragma unroll
                 for (int x = 0; x < KT / 32; ++x)
-                    mask_scores<T>(s[x], p, j + 32 * x, static_cast<unsigned>(gone >> (32 * x + 4 * half)), last, mrow,
-                                   half, whole);
+                    mask_scores<T>(s[x], p.c,
+                                   bits[x] | static_cast<uint32_t>(gone >> (32 * x)) | beyond(j + 32 * x, last),
+                                   values ? mrow + j + 32 * x : nullptr, p.K - j - 32 * x, half);
             }
             float mt = kNegInf;
 #pragma unroll
@@ -266,11 +277,21 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
         return;
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    T* const out = static_cast<T*>(p.out) + ((static_cast<int64_t>(b) * p.Q + i) * p.H + h) * p.D;
+    const int64_t out_at = ((static_cast<int64_t>(b) * p.Q + i) * p.H + h) * p.D;
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
+    for (int d = 0; d < ND; ++d) {
+        o[d] *= inv;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) store4<T>(out, 32 * d + 8 * x + 4 * half, p.D, vec_out, o[d], 4 * x, inv);
+        for (int x = 0; x < 4; ++x)
+            store4<T>(static_cast<T*>(p.out) + out_at, 32 * d + 8 * x + 4 * half, p.D, vec_out, o[d], 4 * x, 1.f);
+        if (sizeof(T) == 2 && p.out_low != nullptr) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[d][e] -= static_cast<float>(static_cast<T>(o[d][e]));
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                store4<T>(static_cast<T*>(p.out_low) + out_at, 32 * d + 8 * x + 4 * half, p.D, vec_out, o[d], 4 * x, 1.f);
+        }
+    }
     if (p.stats != nullptr && half == 0) {
         float* const st = static_cast<float*>(p.stats) + 2 * row;
         st[0] = l == 0.f ? 0.f : m;
@@ -278,34 +299,55 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
     }
 }
 
-// Joins the key ranges of each row: a wavefront a row, lanes over its channels.
+// Joins the key ranges of each row: a workgroup a row. The ranges' factors 2^(m_s - m) / l go to LDS first, then 256 / W
+// groups of W threads, W the channels rounded up to a power of two, each add every group's share of the ranges.
+constexpr int kJoinRanges = 1024;  // most ranges of a row (shape_of)
 template <typename T>
-__global__ __launch_bounds__(64) void attn_join_kernel(AttnParams p, Split sp) {
-    const int lane = threadIdx.x;
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p, Split sp, int wide) {
+    __shared__ float factor[kJoinRanges], part[256], best[4], total[4];
+    const int t = threadIdx.x, lane = t % kWave, wave = t / kWave;
     const int64_t row = blockIdx.x, rows = static_cast<int64_t>(p.B) * p.H * p.Q;
     float m = kNegInf;
-    for (int s = lane; s < sp.n; s += kWave) m = __builtin_fmaxf(m, sp.ml[2 * (s * rows + row)]);
+    for (int s = t; s < sp.n; s += 256) m = __builtin_fmaxf(m, sp.ml[2 * (s * rows + row)]);
 #pragma unroll
     for (int x = 32; x > 0; x >>= 1) m = __builtin_fmaxf(m, xor_lane(m, x));
+    if (lane == 0) best[wave] = m;
+    __syncthreads();
+    m = __builtin_fmaxf(__builtin_fmaxf(best[0], best[1]), __builtin_fmaxf(best[2], best[3]));
     float l = 0.f;
-    for (int s = lane; s < sp.n; s += kWave) {
+    for (int s = t; s < sp.n; s += 256) {
         const float* ml = sp.ml + 2 * (s * rows + row);
-        if (ml[0] != kNegInf) l += ml[1] * __builtin_amdgcn_exp2f(ml[0] - m);
+        const float f = ml[0] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(ml[0] - m);
+        factor[s] = f;
+        l = fmaf(ml[1], f, l);
     }
     l = wave_sum(l);
+    if (lane == 0) total[wave] = l;
+    __syncthreads();
+    l = (total[0] + total[1]) + (total[2] + total[3]);
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int64_t i = row % p.Q, h = row / p.Q % p.H, b = row / p.Q / p.H;
-    T* const out = static_cast<T*>(p.out) + ((b * p.Q + i) * p.H + h) * p.D;
-    for (int d = lane; d < p.D; d += kWave) {
-        float o = 0.f;
-        for (int s = 0; s < sp.n; ++s) {
-            const int64_t part = s * rows + row;
-            const float ms = sp.ml[2 * part];
-            if (ms != kNegInf) o = fmaf(sp.o[part * p.D + d], __builtin_amdgcn_exp2f(ms - m), o);
+    const int64_t out_at = ((b * p.Q + i) * p.H + h) * p.D;
+    const int d = t % wide, group = t / wide, groups = 256 / wide;
+    float o = 0.f;
+    if (d < p.D) {
+#pragma unroll 4
+        for (int s = group; s < sp.n; s += groups) {
+            const float f = factor[s];
+            if (f != 0.f) o = fmaf(sp.o[(s * rows + row) * p.D + d], f, o);
         }
-        out[d] = static_cast<T>(o * inv);
     }
-    if (p.stats != nullptr && lane == 0) {
+    part[t] = o;
+    __syncthreads();
+    if (group == 0 && d < p.D) {
+        for (int g = 1; g < groups; ++g) o += part[g * wide + d];
+        o *= inv;
+        const T v = static_cast<T>(o);
+        static_cast<T*>(p.out)[out_at + d] = v;
+        if (sizeof(T) == 2 && p.out_low != nullptr)
+            static_cast<T*>(p.out_low)[out_at + d] = static_cast<T>(o - static_cast<float>(v));
+    }
+    if (p.stats != nullptr && t == 0) {
         float* const st = static_cast<float*>(p.stats) + 2 * row;
         st[0] = l == 0.f ? 0.f : m;
         st[1] = l == 0.f ? 0.f : __builtin_amdgcn_logf(l) - kShift<T>;
@@ -338,6 +380,7 @@ Shape shape_of(int dtype, const AttnParams& p) {
         int64_t n = (1024 + groups - 1) / groups;
         const int64_t most = (p.K + 511) / 512;
         n = n < most ? n : most;
+        n = n < kJoinRanges ? n : kJoinRanges;
         const int64_t keys = ((p.K + n - 1) / n + 255) / 256 * 256;
         s.keys = static_cast<int>(keys);
         s.n = static_cast<int>((p.K + keys - 1) / keys);
@@ -357,19 +400,22 @@ int run(const AttnParams& p, const Shape& s, const Split& sp, hipStream_t stream
         bytes > 64 * 1024 ? allow_dynamic_lds(reinterpret_cast<const void*>(fn), bytes, done) : hipSuccess;
     if (e != hipSuccess) return set_error(TD_E_LAUNCH, "attention: LDS size: %s", hipGetErrorString(e));
     const int64_t n = static_cast<int64_t>(p.B) * p.Hk * s.tiles * s.n;
-    const bool vec_out = p.D % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % (4 * sizeof(T)) == 0;
+    const bool vec_out = p.D % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.out_low)) %
+                                                 (4 * sizeof(T)) == 0;
     hipLaunchKernelGGL(fn, dim3(xcd_grid(n)), dim3(256), bytes, stream, p, sp, vec_out, s.tiles);
     if (s.n > 1)
-        hipLaunchKernelGGL((attn_join_kernel<T>), dim3(static_cast<unsigned>(p.B) * p.H * p.Q), dim3(64), 0, stream, p,
-                           sp);
+        hipLaunchKernelGGL((attn_join_kernel<T>), dim3(static_cast<unsigned>(p.B) * p.H * p.Q), dim3(256), 0, stream, p,
+                           sp, padded_width(p.D));
     const hipError_t le = hipGetLastError();
     return le == hipSuccess ? 0 : set_error(TD_E_LAUNCH, "attention launch failed: %s", hipGetErrorString(le));
 }
 
 template <typename T, int DP>
 int run_dp(const AttnParams& p, const Shape& s, const Split& sp, hipStream_t stream) {
-    const bool mask = p.mask_type != TD_MASK_NONE;
-    if (!s.vec) return run<T, DP, false, true, false>(p, s, sp, stream);
+    const bool mask = p.mask_type != TD_MASK_NONE && p.K > 0;
+    if (!s.vec)
+        return mask ? run<T, DP, false, true, false>(p, s, sp, stream)
+                    : run<T, DP, false, false, false>(p, s, sp, stream);
     if constexpr (DP * sizeof(T) <= 256)
         if (s.wk)
             return mask ? run<T, DP, true, true, true>(p, s, sp, stream)
@@ -384,12 +430,16 @@ template <typename T>
 int launch_attn_forward_t(int dtype, const AttnParams& p, hipStream_t stream) {
     const Shape s = shape_of(dtype, p);
     const int64_t rows = static_cast<int64_t>(p.B) * p.H * p.Q;
-    const Split sp{s.n, s.keys, static_cast<float*>(p.ws), static_cast<float*>(p.ws) + s.n * rows * p.D};
+    AttnParams q = p;
+    float* const ws = reinterpret_cast<float*>(static_cast<unsigned char*>(p.ws) + plan_mask(q, p.ws));
+    const Split sp{s.n, s.keys, ws, ws + s.n * rows * p.D};
+    const int rc = launch_mask(dtype, q, stream);
+    if (rc != 0) return rc;
     switch (padded_width(p.D)) {
-        case 32: return run_dp<T, 32>(p, s, sp, stream);
-        case 64: return run_dp<T, 64>(p, s, sp, stream);
-        case 128: return run_dp<T, 128>(p, s, sp, stream);
-        default: return run_dp<T, 256>(p, s, sp, stream);
+        case 32: return run_dp<T, 32>(q, s, sp, stream);
+        case 64: return run_dp<T, 64>(q, s, sp, stream);
+        case 128: return run_dp<T, 128>(q, s, sp, stream);
+        default: return run_dp<T, 256>(q, s, sp, stream);
     }
 }
 
@@ -399,7 +449,8 @@ template int launch_attn_forward_t<float>(int, const AttnParams&, hipStream_t);
 int64_t attn_forward_workspace(int dtype, const AttnParams& p) {
     if (dtype == kF64) return 0;
     const Shape s = shape_of(dtype, p);
-    return s.n == 1 ? 0 : static_cast<int64_t>(s.n) * p.B * p.H * p.Q * (p.D + 2) * 4;
+    AttnParams q = p;
+    return plan_mask(q, nullptr) + (s.n == 1 ? 0 : static_cast<int64_t>(s.n) * p.B * p.H * p.Q * (p.D + 2) * 4);
 }
 
 int launch_attn_forward(int dtype, const AttnParams& p, hipStream_t stream) {

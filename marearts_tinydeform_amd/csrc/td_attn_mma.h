@@ -216,29 +216,21 @@ __device__ __forceinline__ float mask_log2(float m) {
     return m == kNegInf ? kNegInf : __builtin_fmaxf(m * kLog2e, kLowest);
 }
 
-// Four consecutive mask entries of a row at key j, `left` of them inside it
-template <typename T>
-__device__ __forceinline__ void mask4_float(const T* m, int left, bool whole, float (&o)[4]) {
-    T v[4];
-    if (whole) {
-        __builtin_memcpy(v, m, sizeof(v));
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = e < left ? m[e] : static_cast<T>(0.f);
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = mask_log2(static_cast<float>(v[e]));
+// Keys j0 .. j0 + 31 beyond `last`, the last key that a query sees, as bits
+__device__ __forceinline__ uint32_t beyond(int j0, int last) {
+    return last < j0 ? ~0u : last - j0 >= 31 ? 0u : ~0u << (last - j0 + 1);
 }
-__device__ __forceinline__ unsigned mask4_bytes(const uint8_t* m, int left, bool whole) {
-    unsigned v = 0;
-    if (whole) {
-        __builtin_memcpy(&v, m, 4);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (e < left) v |= static_cast<unsigned>(m[e]) << (8 * e);
-    }
-    return v;
+
+// What the mask has for one row and 32 keys
+struct MaskWord {
+    uint32_t bits;
+    int kind;
+};
+__device__ __forceinline__ MaskWord mask_word(const AttnParams& p, int b, int h, int i, int word) {
+    if (word >= p.words) return MaskWord{~0u, kMaskAll};
+    const int64_t row = b * p.bs[0] + h * p.bs[1] + i * p.bs[2];
+    const int64_t tile = b * p.kinds_bs[0] + h * p.kinds_bs[1] + (p.bs[2] == 0 ? 0 : i >> 5);
+    return MaskWord{p.bits[row * p.words + word], p.kinds[tile * p.words + word]};
 }
 
 // Elements x .. x + 3 of an accumulator, times `by`, to channels at .. at + 3 of a row of D. vec: whole groups of 4
@@ -258,28 +250,26 @@ __device__ __forceinline__ void store4(T* row, int at, int D, bool vec, const f3
 }
 
 // Scores of 32 keys (rows 8 i + 4 half + e) by 32 rows of the problem (columns), as the scores in base 2 with -inf where
-// a pair is left out: s *= c, plus the mask. `gone`: bit k set for key j0 + k that nobody sees (shifted by 4 half).
-// last: the last key that the lane's row sees (causal; INT32_MAX without). mrow: the mask's row (or null).
+// a pair is left out: s * c, plus the mask's values. `gone`: the lane's bits for its column's 32 keys. values: the mask's
+// row at the first key of the tile, `left` keys inside it, or null.
 template <typename T>
-__device__ __forceinline__ void mask_scores(f32x16& s, const AttnParams& p, int j0, unsigned gone, int last,
-                                            const void* mrow, int half, bool whole) {
+__device__ __forceinline__ void mask_scores(f32x16& s, float c, uint32_t gone, const T* values, int left, int half) {
+    gone >>= 4 * half;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int j = j0 + 8 * i + 4 * half;
         float add[4] = {0.f, 0.f, 0.f, 0.f};
-        unsigned bytes = 0;
-        if (mrow != nullptr) {
-            if (p.mask_type == TD_MASK_FLOAT)
-                mask4_float<T>(static_cast<const T*>(mrow) + j, p.K - j, whole, add);
-            else
-                bytes = mask4_bytes(static_cast<const uint8_t*>(mrow) + j, p.K - j, whole);
+        if (values != nullptr) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int key = 8 * i + 4 * half + e;
+                if (key < left) add[e] = mask_log2(static_cast<float>(values[key]));
+            }
+            __builtin_amdgcn_sched_barrier(0);  // four loads at a time: registers
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const bool out = ((gone >> (8 * i + e)) & 1u) || j + e > last || ((bytes >> (8 * e)) & 0xffu) ||
-                             add[e] == kNegInf;
-            const float t = fmaf(s[4 * i + e], p.c, add[e]);
-            s[4 * i + e] = out ? kNegInf : t;
+            const float t = fmaf(s[4 * i + e], c, add[e]);
+            s[4 * i + e] = (gone >> (8 * i + e)) & 1u ? kNegInf : t;
         }
     }
 }

@@ -51,19 +51,16 @@ class _AttnFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, query, key, value, attn_mask, key_padding_mask, scale, causal):
-        out, stats = _dense.attn_forward(query, key, value, attn_mask, key_padding_mask, scale, causal,
-                                         want_stats=True)
-        ctx.save_for_backward(query, key, value, attn_mask, key_padding_mask, out, stats)
-        ctx.scale, ctx.causal = scale, causal
+        out, tensors, ctx.values = _dense.attn_forward(query, key, value, attn_mask, key_padding_mask, scale, causal,
+                                                       train=True)
+        ctx.save_for_backward(*tensors)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        query, key, value, attn_mask, key_padding_mask, out, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dq, dk, dv = _dense.attn_backward(query, key, value, attn_mask, key_padding_mask, ctx.scale, ctx.causal, out,
-                                          stats, grad_out, need[0], need[1] or need[2])
+        dq, dk, dv = _dense.attn_backward(ctx.saved_tensors, ctx.values, grad_out, need[0], need[1] or need[2])
         return dq, dk if need[1] else None, dv if need[2] else None, None, None, None, None
 
 
@@ -102,16 +99,15 @@ class _LayerNormFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, eps):
-        out, stats = _dense.layer_norm_forward(x, weight, bias, residual, eps, want_stats=True)
-        ctx.save_for_backward(x, weight, residual, stats)
+        out, tensors = _dense.layer_norm_forward(x, weight, bias, residual, eps, train=True)
+        ctx.save_for_backward(*tensors)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        x, weight, residual, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dx, dw, db = _dense.layer_norm_backward(x, weight, residual, stats, grad_out, need[1], need[2])
+        dx, dw, db = _dense.layer_norm_backward(ctx.saved_tensors, grad_out, need[1], need[2])
         return dx if need[0] else None, dw, db, dx if need[3] else None, None
 
 

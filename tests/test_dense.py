@@ -219,7 +219,7 @@ P = 4096  # a stand-in address: these calls end before anything is read
 def packed(dtype=1, kind=0, causal=0, B=2, Q=5, K=7, H=4, Hk=2, D=8, scale=1.0, q=P, k=P, v=P, mask=0, pad=0, out=P,
            stats=P, stride=8):
     return _dense.ATTN_ARGS.pack(dtype, kind, causal, 0, B, Q, K, H, Hk, D, scale, q, k, v, *([8] * 8), stride, mask, 0,
-                                 0, 0, pad, out, stats)
+                                 0, 0, pad, out, stats, 0)
 
 
 @pytest.mark.parametrize('kw,code,message', [

@@ -61,6 +61,34 @@ def test_masks(mask, dtype):
         assert torch.equal(again, out), 'inference and training forward differ'
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('form', ['bool', 'float', 'float with a value'])
+def test_block_masks(form, dtype):
+    """Masks of whole blocks (denoising groups): 32 x 32 tiles with nothing, something and everything masked, for
+    shared and single heads, a mask by head and by batch, more keys than queries and fewer."""
+    g = torch.Generator().manual_seed(3)
+    for size, lead in (((2, 200, 200, 4, 4, 32), (200,)), ((2, 130, 330, 6, 2, 64), (2, 6, 130)),
+                       ((1, 300, 100, 8, 8, 32), (1, 8, 1)), ((2, 100, 100, 12, 4, 32), (2, 1, 100)),
+                       ((2, 70, 600, 4, 1, 128), (1, 4, 70))):
+        say(f'  block mask {form} {size} {lead} {dtype}')
+        q, k, v, go, _ = make_attn(size, dtype)
+        Q, K = size[1], size[2]
+        rows, cols = torch.arange(lead[-1])[:, None] // 48, torch.arange(K)[None, :] // 80
+        mask = ((rows * 7 + cols * 3) % 5 < 2) & (rows != 1)
+        shape = tuple(lead[:-1]) + (lead[-1], K)
+        mask = mask.expand(shape).clone()
+        if len(shape) == 4:
+            mask ^= torch.rand(shape[:2], generator=g)[:, :, None, None] < 0.3
+            mask &= torch.rand(shape[:2], generator=g)[:, :, None, None] < 0.9
+        kw = dict(attn_mask=mask)
+        if form != 'bool':
+            kw['attn_mask'] = torch.zeros(shape, dtype=dtype).masked_fill(mask, float('-inf'))
+            if form != 'float':
+                kw['attn_mask'][..., ::70, 5::64] += 1.25
+        out, grads = run(q, k, v, go, kw)
+        check_attn(dtype, q, k, v, go, kw, out, grads)
+
+
 @pytest.mark.parametrize('mask', ['none', 'bool', 'float', 'lowest', 'all'])
 def test_float64(mask):
     for size in [(2, 33, 70, 4, 2, 36), (1, 1, 65, 2, 2, 128)]:
@@ -254,7 +282,10 @@ def test_c_abi_writes_its_buffers_and_nothing_else(dtype):
         bufs = [fenced(B * Q * H * D, dtype), fenced(B * H * Q * 2, acc), fenced(B * Q * H * D, dtype),
                 fenced(B * K * Hk * D, dtype), fenced(B * K * Hk * D, dtype)]
         out, stats, dq, dk, dv = (b[1] for b in bufs)
-        args = _dense._pack(q, k, v, None, 0, (0, 0, 0), None, D ** -0.5, False, out, stats)
+        low = fenced(B * Q * H * D, dtype)
+        bufs.append(low)
+        args = _dense._pack(q, k, v, None, 0, (0, 0, 0), None, D ** -0.5, False, out, stats,
+                            None if dtype == torch.float32 else low[1])
         need = lib.td_attn_forward_workspace(args)
         w1 = fenced(max(need, 4) // 4, torch.float32)
         assert lib.td_attn_forward(args, w1[1].data_ptr(), need, None) == 0
