@@ -132,23 +132,55 @@ template <typename T, int DP, bool WK>
 constexpr int dq_key_tile() {
     return WK || DP * static_cast<int>(sizeof(T)) > 128 ? 32 : 64;
 }
-// Wavefronts a SIMD that the registers leave room for without spills
-template <typename T, int DP, bool WK, bool SLOW>
+// Wavefronts a SIMD that the registers leave room for with few spills or none
+template <typename T, int DP, bool SLOW>
 constexpr int dq_min_waves() {
     constexpr int bytes = DP * static_cast<int>(sizeof(T));
-    return bytes <= 64 ? (SLOW ? 2 : 3) : bytes <= 128 || (bytes <= 256 && !WK) ? 2 : 1;
+    return bytes <= 64 ? (SLOW ? 2 : 3) : bytes <= 256 ? 2 : 1;
+}
+
+// A sum over many keys (dQ) or rows (dK, dV) of few outputs is split over n workgroups, whose parts, float32 in the
+// outputs' order, sum_parts_kernel adds.
+struct Parts {
+    int n;
+    float *a, *b;  // [n][outputs]: dQ, or dK and dV
+    int64_t outputs;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void sum_parts_kernel(const float* __restrict__ part, int n, int64_t outputs,
+                                                        T* __restrict__ out) {
+    const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+    if (i >= outputs) return;
+    const bool whole = i + 4 <= outputs && outputs % 4 == 0;
+    f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (whole) {
+#pragma unroll 4
+        for (int k = 0; k < n; ++k) s += *reinterpret_cast<const f32x4*>(part + k * outputs + i);
+    } else {
+        for (int k = 0; k < n; ++k)
+            for (int e = 0; e < 4 && i + e < outputs; ++e) s[e] += part[k * outputs + i + e];
+    }
+    for (int e = 0; e < 4 && i + e < outputs; ++e) out[i + e] = static_cast<T>(s[e]);
+}
+
+template <typename T>
+void sum_parts(const float* part, const Parts& parts, void* out, hipStream_t stream) {
+    hipLaunchKernelGGL((sum_parts_kernel<T>), dim3(static_cast<unsigned>((parts.outputs + 1023) / 1024)), dim3(256), 0,
+                       stream, part, parts.n, parts.outputs, static_cast<T*>(out));
 }
 
 template <typename T, int DP, bool WK, bool MASK, bool VEC>
-__global__ __launch_bounds__(256, (dq_min_waves<T, DP, WK, MASK>())) void attn_dq_kernel(AttnParams p, RowInfo info,
-                                                                                    bool vec_out, int tiles) {
+__global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dq_kernel(AttnParams p, RowInfo info,
+                                                                                    Parts parts, bool vec_out,
+                                                                                    int tiles) {
     using R = TileRows<T, DP>;
     constexpr int KT = dq_key_tile<T, DP, WK>(), NT = WK ? 64 : 256, ND = DP / 32;
     constexpr int kTile = KT * R::kPitch;
     extern __shared__ __align__(16) unsigned char lds[];
-    const int id = xcd_order(static_cast<int>(blockIdx.x), p.B * p.Hk * tiles);
+    const int id = xcd_order(static_cast<int>(blockIdx.x), p.B * p.Hk * tiles * parts.n);
     if (id < 0) return;
-    const int tile = tiles - 1 - id % tiles, bh = id / tiles;  // causal: the long ones first
+    const int split = id % parts.n, tile = tiles - 1 - id / parts.n % tiles, bh = id / parts.n / tiles;  // causal: long first
     const int b = bh / p.Hk, hk = bh % p.Hk;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
     const int lane = threadIdx.x % kWave, half = lane >> 5;
@@ -210,6 +242,11 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, WK, MASK>())) void attn_d
     constexpr int step = WK ? 4 * KT : KT;
     constexpr uint64_t all = KT == 64 ? ~uint64_t{0} : (uint64_t{1} << (KT & 63)) - 1;
     int64_t j0 = WK ? wave * KT : 0;
+    if (parts.n > 1) {
+        const int64_t each = (static_cast<int64_t>(kend > 0 ? kend : 0) + parts.n * step - 1) / (parts.n * step) * step;
+        j0 += split * each;
+        kend = (split + 1) * each < kend ? static_cast<int>((split + 1) * each) : kend;
+    }
     uint64_t gone = __ballot(pad_byte(j0)), gone_next;
     MaskWord mw[KT / 32] = {};
     auto fetch = [&](int64_t at, uint64_t g) {
@@ -316,11 +353,16 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, WK, MASK>())) void attn_d
     }
     if (!live) return;
     const float back = static_cast<float>(p.scale) / ds_scale * (kScaled<T> ? 0x1p-15f : 1.f);
-    T* const out = static_cast<T*>(p.dq) + out_at;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) store4<T>(out, 32 * d + 8 * x + 4 * half, p.D, vec_out, dq[d], 4 * x, back);
+        for (int x = 0; x < 4; ++x) {
+            const int at = 32 * d + 8 * x + 4 * half;
+            if (parts.n > 1)
+                store4<float>(parts.a + split * parts.outputs + out_at, at, p.D, vec_out, dq[d], 4 * x, back);
+            else
+                store4<T>(static_cast<T*>(p.dq) + out_at, at, p.D, vec_out, dq[d], 4 * x, back);
+        }
 }
 
 // dK and dV. WK false: four wavefronts of 32 keys each share the row tiles. WK true: 32 keys a workgroup and the row tiles
@@ -343,17 +385,19 @@ constexpr int dkv_row_bytes() {
 }
 
 template <typename T, int DP, bool WK, bool MASK, bool VEC>
-__global__ __launch_bounds__(256, (dq_min_waves<T, DP, WK, MASK>())) void attn_dkv_kernel(AttnParams p, RowInfo info,
-                                                                                     bool vec_out, int tiles) {
+__global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dkv_kernel(AttnParams p, RowInfo info,
+                                                                                     Parts parts, bool vec_out,
+                                                                                     int tiles) {
     using R = TileRows<T, DP>;
     constexpr int RT = dkv_row_tile<T, DP, WK>(), NT = WK ? 64 : 256, ND = DP / 32;
     constexpr int kTile = RT * R::kPitch;
     constexpr int KW = WK ? 1 : 4;  // words of 32 keys that the workgroup's keys have
     constexpr int kArea = 2 * kTile + RT * dkv_row_bytes<WK, MASK>();
     extern __shared__ __align__(16) unsigned char lds[];
-    const int id = xcd_order(static_cast<int>(blockIdx.x), p.B * p.Hk * tiles);
+    const int id = xcd_order(static_cast<int>(blockIdx.x), p.B * p.Hk * tiles * parts.n);
     if (id < 0) return;
-    const int tile = id % tiles, bh = id / tiles;  // causal: the first keys are seen by the most rows
+    const int split = id % parts.n, tile = id / parts.n % tiles, bh = id / parts.n / tiles;  // causal: the first keys are
+                                                                                            // seen by the most rows
     const int b = bh / p.Hk, hk = bh % p.Hk;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
     const int lane = threadIdx.x % kWave, half = lane >> 5;
@@ -466,9 +510,15 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, WK, MASK>())) void attn_d
     for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f32x16{0.f};
 
     constexpr int step = WK ? 4 * RT : RT;
+    int64_t rend = p.rows;
+    if (parts.n > 1) {
+        const int64_t each = (p.rows > r0 ? p.rows - r0 + parts.n * step - 1 : 0) / (parts.n * step) * step;
+        r0 += split * each;
+        rend = r0 + each < rend ? r0 + each : rend;
+    }
     if (WK) r0 += wave * RT;
-    if (r0 < p.rows) fetch(r0);
-    for (; r0 < p.rows; r0 += step) {
+    if (r0 < rend) fetch(r0);
+    for (; r0 < rend; r0 += step) {
         if (!WK) __syncthreads();
         qs.store(q_lds, t);
         gs.store(g_lds, t);
@@ -489,7 +539,7 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, WK, MASK>())) void attn_d
             wave_sync();
         else
             __syncthreads();
-        if (r0 + step < p.rows) fetch(r0 + step);
+        if (r0 + step < rend) fetch(r0 + step);
         if (any && r0 + RT > wfirst_row) {
             const uint32_t* const my_words = w_lds + (WK ? 0 : wave * RT);
 #pragma unroll
@@ -603,39 +653,59 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, WK, MASK>())) void attn_d
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
             const int c = 32 * d + 8 * x + 4 * half;
-            store4<T>(static_cast<T*>(p.dk) + at, c, p.D, vec_out, dk[d], 4 * x, back);
-            store4<T>(static_cast<T*>(p.dv) + at, c, p.D, vec_out, dv[d], 4 * x, pv);
+            if (parts.n > 1) {
+                store4<float>(parts.a + split * parts.outputs + at, c, p.D, vec_out, dk[d], 4 * x, back);
+                store4<float>(parts.b + split * parts.outputs + at, c, p.D, vec_out, dv[d], 4 * x, pv);
+            } else {
+                store4<T>(static_cast<T*>(p.dk) + at, c, p.D, vec_out, dk[d], 4 * x, back);
+                store4<T>(static_cast<T*>(p.dv) + at, c, p.D, vec_out, dv[d], 4 * x, pv);
+            }
         }
     }
 }
 
 struct BackShape {
     bool vec, wk_q, wk_k;
-    int q_tiles, k_tiles;
+    int q_tiles, k_tiles, q_parts, k_parts;
 };
 
-BackShape back_shape(int dtype, const AttnParams& p) {
+bool back_vec(int dtype, const AttnParams& p) {
     const int elem = elem_size(dtype);
     auto ok = [&](const void* ptr, const int64_t (&s)[3]) {
         return reinterpret_cast<uintptr_t>(ptr) % 16 == 0 && s[0] * elem % 16 == 0 && s[1] * elem % 16 == 0 &&
                s[2] * elem % 16 == 0 && s[1] < (int64_t{1} << 31) / (128 * elem) &&
                s[2] < (int64_t{1} << 31) / (int64_t{2} * p.G * elem);
     };
+    return p.D * elem % 16 == 0 && ok(p.q, p.qs) && ok(p.k, p.ks) && ok(p.v, p.vs) &&
+           reinterpret_cast<uintptr_t>(p.go) % 16 == 0 &&
+           static_cast<int64_t>(p.H) * p.D < (int64_t{1} << 31) / (128 * elem);
+}
+
+// Workgroups of 128 rows (keys) that share tiles, when they fill the GPU twice; else of 32 rows (keys) with the others'
+// tiles over the wavefronts, which needs no second launch, for heads whose private tiles fit in the registers. Where that
+// still leaves CUs without work and the loops are long, parts.
+BackShape back_shape(int dtype, const AttnParams& p, bool vec) {
     BackShape s{};
-    s.vec = p.D * elem % 16 == 0 && ok(p.q, p.qs) && ok(p.k, p.ks) && ok(p.v, p.vs) &&
-            reinterpret_cast<uintptr_t>(p.go) % 16 == 0 &&
-            static_cast<int64_t>(p.H) * p.D < (int64_t{1} << 31) / (128 * elem);
+    s.vec = vec;
     const int64_t heads = static_cast<int64_t>(p.B) * p.Hk;
-    const bool can = s.vec && padded_width(p.D) * elem <= 256;
-    s.wk_q = can && heads * ((p.rows + 127) / 128) < 512;
-    s.wk_k = can && heads * ((p.K + 127) / 128) < 512;
-    s.q_tiles = s.wk_q ? (p.rows + 31) / 32 : (p.rows + 127) / 128;
-    s.k_tiles = s.wk_k ? (p.K + 31) / 32 : (p.K + 127) / 128;
+    const bool can = vec && padded_width(p.D) * elem_size(dtype) <= 128;
+    auto shape = [&](int n, int over, bool& wk, int& tiles, int& parts) {
+        wk = can && heads * ((n + 127) / 128) < 512;
+        tiles = wk ? (n + 31) / 32 : (n + 127) / 128;
+        parts = 1;
+        const int64_t groups = heads * tiles;
+        if (groups == 0 || groups >= 384) return;
+        const int64_t want = (1024 + groups - 1) / groups, most = over / 512;  // 4 steps of 4 x 32 or 16 of 32 a part
+        parts = static_cast<int>(want < most ? want : most);
+        parts = parts < 1 ? 1 : parts;
+    };
+    shape(p.rows, p.K, s.wk_q, s.q_tiles, s.q_parts);
+    shape(p.K, p.rows, s.wk_k, s.k_tiles, s.k_parts);
     return s;
 }
 
 template <typename T, int DP, bool WK, bool MASK, bool VEC>
-int run_dq(const AttnParams& p, const BackShape& s, const RowInfo& info, hipStream_t stream) {
+int run_dq(const AttnParams& p, const BackShape& s, const RowInfo& info, float* ws, hipStream_t stream) {
     static std::atomic<uint64_t> done{0};
     constexpr int tile = 2 * dq_key_tile<T, DP, WK>() * TileRows<T, DP>::kPitch;
     constexpr int join = 2 * 32 * (DP + 4) * 4;
@@ -646,13 +716,15 @@ int run_dq(const AttnParams& p, const BackShape& s, const RowInfo& info, hipStre
         bytes > 64 * 1024 ? allow_dynamic_lds(reinterpret_cast<const void*>(fn), bytes, done) : hipSuccess;
     if (e != hipSuccess) return set_error(TD_E_LAUNCH, "attention backward: LDS size: %s", hipGetErrorString(e));
     const bool vec_out = p.D % 4 == 0 && reinterpret_cast<uintptr_t>(p.dq) % (4 * sizeof(T)) == 0;
-    const int64_t n = static_cast<int64_t>(p.B) * p.Hk * s.q_tiles;
-    hipLaunchKernelGGL(fn, dim3(xcd_grid(n)), dim3(256), bytes, stream, p, info, vec_out, s.q_tiles);
+    const Parts parts{s.q_parts, ws, nullptr, static_cast<int64_t>(p.B) * p.Q * p.H * p.D};
+    const int64_t n = static_cast<int64_t>(p.B) * p.Hk * s.q_tiles * parts.n;
+    hipLaunchKernelGGL(fn, dim3(xcd_grid(n)), dim3(256), bytes, stream, p, info, parts, vec_out, s.q_tiles);
+    if (parts.n > 1) sum_parts<T>(parts.a, parts, p.dq, stream);
     return 0;
 }
 
 template <typename T, int DP, bool WK, bool MASK, bool VEC>
-int run_dkv(const AttnParams& p, const BackShape& s, const RowInfo& info, hipStream_t stream) {
+int run_dkv(const AttnParams& p, const BackShape& s, const RowInfo& info, float* ws, hipStream_t stream) {
     static std::atomic<uint64_t> done{0};
     constexpr int RT = dkv_row_tile<T, DP, WK>(), area = 2 * RT * TileRows<T, DP>::kPitch + RT * dkv_row_bytes<WK, MASK>();
     constexpr int join = 2 * 32 * (DP + 4) * 4;
@@ -665,36 +737,42 @@ int run_dkv(const AttnParams& p, const BackShape& s, const RowInfo& info, hipStr
     if (e != hipSuccess) return set_error(TD_E_LAUNCH, "attention backward: LDS size: %s", hipGetErrorString(e));
     const bool vec_out = p.D % 4 == 0 && reinterpret_cast<uintptr_t>(p.dk) % (4 * sizeof(T)) == 0 &&
                          reinterpret_cast<uintptr_t>(p.dv) % (4 * sizeof(T)) == 0;
-    const int64_t n = static_cast<int64_t>(p.B) * p.Hk * s.k_tiles;
-    hipLaunchKernelGGL(fn, dim3(xcd_grid(n)), dim3(256), bytes, stream, p, info, vec_out, s.k_tiles);
+    const int64_t outputs = static_cast<int64_t>(p.B) * p.K * p.Hk * p.D;
+    const Parts parts{s.k_parts, ws, ws + s.k_parts * outputs, outputs};
+    const int64_t n = static_cast<int64_t>(p.B) * p.Hk * s.k_tiles * parts.n;
+    hipLaunchKernelGGL(fn, dim3(xcd_grid(n)), dim3(256), bytes, stream, p, info, parts, vec_out, s.k_tiles);
+    if (parts.n > 1) {
+        sum_parts<T>(parts.a, parts, p.dk, stream);
+        sum_parts<T>(parts.b, parts, p.dv, stream);
+    }
     return 0;
 }
 
 template <typename T, int DP>
-int run_dp(const AttnParams& p, const BackShape& s, const RowInfo& info, hipStream_t stream) {
+int run_dp(const AttnParams& p, const BackShape& s, const RowInfo& info, float* ws, hipStream_t stream) {
     const bool mask = p.mask_type != TD_MASK_NONE && p.K > 0;
     int rc = 0;
     if (p.dq != nullptr && p.rows > 0) {
         if (!s.vec)
-            rc = mask ? run_dq<T, DP, false, true, false>(p, s, info, stream)
-                      : run_dq<T, DP, false, false, false>(p, s, info, stream);
+            rc = mask ? run_dq<T, DP, false, true, false>(p, s, info, ws, stream)
+                      : run_dq<T, DP, false, false, false>(p, s, info, ws, stream);
         else if (!s.wk_q)
-            rc = mask ? run_dq<T, DP, false, true, true>(p, s, info, stream)
-                      : run_dq<T, DP, false, false, true>(p, s, info, stream);
-        else if constexpr (DP * sizeof(T) <= 256)
-            rc = mask ? run_dq<T, DP, true, true, true>(p, s, info, stream)
-                      : run_dq<T, DP, true, false, true>(p, s, info, stream);
+            rc = mask ? run_dq<T, DP, false, true, true>(p, s, info, ws, stream)
+                      : run_dq<T, DP, false, false, true>(p, s, info, ws, stream);
+        else if constexpr (DP * sizeof(T) <= 128)
+            rc = mask ? run_dq<T, DP, true, true, true>(p, s, info, ws, stream)
+                      : run_dq<T, DP, true, false, true>(p, s, info, ws, stream);
     }
     if (rc == 0 && p.dk != nullptr && p.K > 0) {
         if (!s.vec)
-            rc = mask ? run_dkv<T, DP, false, true, false>(p, s, info, stream)
-                      : run_dkv<T, DP, false, false, false>(p, s, info, stream);
+            rc = mask ? run_dkv<T, DP, false, true, false>(p, s, info, ws, stream)
+                      : run_dkv<T, DP, false, false, false>(p, s, info, ws, stream);
         else if (!s.wk_k)
-            rc = mask ? run_dkv<T, DP, false, true, true>(p, s, info, stream)
-                      : run_dkv<T, DP, false, false, true>(p, s, info, stream);
-        else if constexpr (DP * sizeof(T) <= 256)
-            rc = mask ? run_dkv<T, DP, true, true, true>(p, s, info, stream)
-                      : run_dkv<T, DP, true, false, true>(p, s, info, stream);
+            rc = mask ? run_dkv<T, DP, false, true, true>(p, s, info, ws, stream)
+                      : run_dkv<T, DP, false, false, true>(p, s, info, ws, stream);
+        else if constexpr (DP * sizeof(T) <= 128)
+            rc = mask ? run_dkv<T, DP, true, true, true>(p, s, info, ws, stream)
+                      : run_dkv<T, DP, true, false, true>(p, s, info, ws, stream);
     }
     return rc;
 }
@@ -708,13 +786,21 @@ RowInfo info_of(const AttnParams& p, void* at) {
     return r;
 }
 
+// A multiple of 16
+int64_t info_bytes(int dtype, const AttnParams& p) {
+    const RowInfo r = info_of(p, nullptr);
+    const int64_t heads = static_cast<int64_t>(p.B) * p.Hk;
+    return heads * p.rows * 16 + (dtype == kF16 ? (heads * (r.blocks + r.key_blocks) * 4 + 15) / 16 * 16 : 0);
+}
+
 }  // namespace
 
 template <typename T>
 int launch_attn_backward_t(int dtype, const AttnParams& given, hipStream_t stream) {
     AttnParams p = given;
-    const BackShape s = back_shape(dtype, p);
+    const BackShape s = back_shape(dtype, p, back_vec(dtype, p));
     const RowInfo info = info_of(p, static_cast<unsigned char*>(p.ws) + plan_mask(p, p.ws));
+    float* const ws = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(info.rows) + info_bytes(dtype, p));
     int rc = launch_mask(dtype, p, stream);
     if (rc != 0) return rc;
     const int64_t blocks =
@@ -724,10 +810,10 @@ int launch_attn_backward_t(int dtype, const AttnParams& given, hipStream_t strea
     if (blocks > 0)
         hipLaunchKernelGGL((attn_info_kernel<T>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, p, info, vec);
     switch (padded_width(p.D)) {
-        case 32: rc = run_dp<T, 32>(p, s, info, stream); break;
-        case 64: rc = run_dp<T, 64>(p, s, info, stream); break;
-        case 128: rc = run_dp<T, 128>(p, s, info, stream); break;
-        default: rc = run_dp<T, 256>(p, s, info, stream);
+        case 32: rc = run_dp<T, 32>(p, s, info, ws, stream); break;
+        case 64: rc = run_dp<T, 64>(p, s, info, ws, stream); break;
+        case 128: rc = run_dp<T, 128>(p, s, info, ws, stream); break;
+        default: rc = run_dp<T, 256>(p, s, info, ws, stream);
     }
     if (rc != 0) return rc;
     const hipError_t e = hipGetLastError();
@@ -738,11 +824,17 @@ int launch_attn_backward_t(int dtype, const AttnParams& given, hipStream_t strea
 template int launch_attn_backward_t<float>(int, const AttnParams&, hipStream_t);
 
 int64_t attn_backward_workspace(int dtype, const AttnParams& p) {
-    const int64_t rows = static_cast<int64_t>(p.B) * p.H * p.Q;
-    if (dtype == kF64) return rows * 8;
-    const RowInfo r = info_of(p, nullptr);
+    if (dtype == kF64) return static_cast<int64_t>(p.B) * p.H * p.Q * 8;
+    int64_t parts = 0;  // dQ's and then dK's and dV's
+    for (const bool vec : {false, true}) {  // the gradients' alignment is not known yet
+        const BackShape s = back_shape(dtype, p, vec);
+        const int64_t q = s.q_parts > 1 ? static_cast<int64_t>(s.q_parts) * p.B * p.Q * p.H * p.D : 0;
+        const int64_t k = s.k_parts > 1 ? 2 * static_cast<int64_t>(s.k_parts) * p.B * p.K * p.Hk * p.D : 0;
+        parts = parts > q ? parts : q;
+        parts = parts > k ? parts : k;
+    }
     AttnParams q = p;
-    return plan_mask(q, nullptr) + rows * 16 + (dtype == kF16 ? static_cast<int64_t>(p.B) * p.Hk * (r.blocks + r.key_blocks) * 4 : 0);
+    return plan_mask(q, nullptr) + info_bytes(dtype, p) + parts * 4;
 }
 
 int launch_attn_backward(int dtype, const AttnParams& p, hipStream_t stream) {

@@ -12,7 +12,7 @@ ATTN_SIZES = [
     (2, 129, 65, 2, 2, 32), (1, 40, 257, 4, 4, 64), (1, 37, 300, 2, 2, 128), (1, 50, 130, 2, 2, 16),
     (2, 31, 45, 2, 2, 1), (1, 20, 70, 3, 3, 7), (2, 45, 100, 2, 2, 36), (1, 35, 90, 2, 2, 80), (1, 21, 75, 2, 2, 96),
     (1, 40, 70, 1, 1, 129), (1, 33, 150, 2, 2, 256), (2, 1, 1000, 16, 4, 64), (1, 70, 90, 8, 1, 32),
-    (2, 43, 52, 6, 2, 40), (3, 2, 200, 12, 4, 32), (1, 7, 2500, 2, 1, 64),
+    (2, 43, 52, 6, 2, 40), (3, 2, 200, 12, 4, 32), (1, 7, 2500, 2, 1, 64), (1, 2500, 40, 4, 2, 32), (1, 1300, 70, 3, 1, 128), (1, 40, 1100, 1, 1, 50),
 ]
 MASKS = ['none', 'bool', 'bool4', 'float', 'float4', 'lowest', 'padding', 'causal', 'all']
 
