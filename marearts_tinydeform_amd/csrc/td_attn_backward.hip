@@ -139,37 +139,60 @@ constexpr int dq_min_waves() {
     return bytes <= 64 ? (SLOW ? 2 : 3) : bytes <= 256 ? 2 : 1;
 }
 
-// A sum over many keys (dQ) or rows (dK, dV) of few outputs is split over n workgroups, whose parts, float32 in the
-// outputs' order, sum_parts_kernel adds.
+// Sums over many keys (dQ) or rows (dK, dV) that are split over workgroups (TileSplit) leave float32 parts, which
+// sum_parts_kernel adds in their order.
 struct Parts {
-    int n;
-    float *a, *b;  // [n][outputs]: dQ, or dK and dV
-    int64_t outputs;
+    TileSplit t;
+    float *a, *b;  // dQ, or dK and dV: [..][rows of a tile][D]
 };
 
+// Four channels of a row of a split tile a thread. keys: the rows are keys (dK, dV), else the problem's rows (dQ).
 template <typename T>
-__global__ __launch_bounds__(256) void sum_parts_kernel(const float* __restrict__ part, int n, int64_t outputs,
-                                                        T* __restrict__ out) {
-    const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
-    if (i >= outputs) return;
-    const bool whole = i + 4 <= outputs && outputs % 4 == 0;
-    f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (whole) {
+__global__ __launch_bounds__(256) void sum_parts_kernel(AttnParams p, TileSplit t, const float* __restrict__ part,
+                                                        T* __restrict__ out, int quads, int tile_rows, int tiles,
+                                                        bool keys, bool vec) {
+    const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int d = static_cast<int>(id % quads) * 4;
+    const int64_t at = id / quads;
+    const int left = static_cast<int>(at / tile_rows), row = static_cast<int>(at % tile_rows);
+    if (left >= t.total - t.whole || d >= p.D) return;
+    const int tile = t.whole + left, bh = tile / tiles, b = bh / p.Hk, hk = bh % p.Hk;
+    const int r = (keys ? tile % tiles : tiles - 1 - tile % tiles) * tile_rows + row;
+    if (r >= (keys ? p.K : p.rows)) return;
+    const float* at0 = part + (static_cast<int64_t>(left) * t.n * tile_rows + row) * p.D;
+    const int64_t step = static_cast<int64_t>(tile_rows) * p.D;
+    f32x16 s = f32x16{0.f};
 #pragma unroll 4
-        for (int k = 0; k < n; ++k) s += *reinterpret_cast<const f32x4*>(part + k * outputs + i);
-    } else {
-        for (int k = 0; k < n; ++k)
-            for (int e = 0; e < 4 && i + e < outputs; ++e) s[e] += part[k * outputs + i + e];
+    for (int k = 0; k < t.n; ++k) {
+        const float* from = at0 + k * step + d;
+        if (vec) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(from);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] += v[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (d + e < p.D) s[e] += from[e];
+        }
     }
-    for (int e = 0; e < 4 && i + e < outputs; ++e) out[i + e] = static_cast<T>(s[e]);
+    int64_t to;
+    if (keys) {
+        to = (static_cast<int64_t>(b) * p.K + r) * p.Hk + hk;
+    } else {
+        const int i = static_cast<int>(fast_div(p.gdiv, static_cast<uint32_t>(r)));
+        to = (static_cast<int64_t>(b) * p.Q + i) * p.H + hk * p.G + r - i * p.G;
+    }
+    store4<T>(out + to * p.D, d, p.D, vec && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(T)) == 0, s, 0, 1.f);
 }
 
 template <typename T>
-void sum_parts(const float* part, const Parts& parts, void* out, hipStream_t stream) {
-    hipLaunchKernelGGL((sum_parts_kernel<T>), dim3(static_cast<unsigned>((parts.outputs + 1023) / 1024)), dim3(256), 0,
-                       stream, part, parts.n, parts.outputs, static_cast<T*>(out));
+void sum_parts(const AttnParams& p, const TileSplit& t, const float* part, void* out, int tile_rows, int tiles, bool keys,
+               hipStream_t stream) {
+    const int quads = (p.D + 3) / 4;
+    const int64_t threads = static_cast<int64_t>(t.total - t.whole) * tile_rows * quads;
+    hipLaunchKernelGGL((sum_parts_kernel<T>), dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, stream, p, t,
+                       part, static_cast<T*>(out), quads, tile_rows, tiles, keys, p.D % 4 == 0);
 }
-
 template <typename T, int DP, bool WK, bool MASK, bool VEC>
 __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dq_kernel(AttnParams p, RowInfo info,
                                                                                     Parts parts, bool vec_out,
@@ -178,9 +201,9 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dq_ke
     constexpr int KT = dq_key_tile<T, DP, WK>(), NT = WK ? 64 : 256, ND = DP / 32;
     constexpr int kTile = KT * R::kPitch;
     extern __shared__ __align__(16) unsigned char lds[];
-    const int id = xcd_order(static_cast<int>(blockIdx.x), p.B * p.Hk * tiles * parts.n);
-    if (id < 0) return;
-    const int split = id % parts.n, tile = tiles - 1 - id / parts.n % tiles, bh = id / parts.n / tiles;  // causal: long first
+    const TileWork work = tile_work(parts.t);
+    if (work.tile < 0) return;
+    const int tile = tiles - 1 - work.tile % tiles, bh = work.tile / tiles;  // causal: the long ones first
     const int b = bh / p.Hk, hk = bh % p.Hk;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
     const int lane = threadIdx.x % kWave, half = lane >> 5;
@@ -242,10 +265,10 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dq_ke
     constexpr int step = WK ? 4 * KT : KT;
     constexpr uint64_t all = KT == 64 ? ~uint64_t{0} : (uint64_t{1} << (KT & 63)) - 1;
     int64_t j0 = WK ? wave * KT : 0;
-    if (parts.n > 1) {
-        const int64_t each = (static_cast<int64_t>(kend > 0 ? kend : 0) + parts.n * step - 1) / (parts.n * step) * step;
-        j0 += split * each;
-        kend = (split + 1) * each < kend ? static_cast<int>((split + 1) * each) : kend;
+    if (work.parts > 1) {
+        const int64_t n = work.parts, each = ((kend > 0 ? kend : 0) + n * step - 1) / (n * step) * step;
+        j0 += work.part * each;
+        kend = (work.part + 1) * each < kend ? static_cast<int>((work.part + 1) * each) : kend;
     }
     uint64_t gone = __ballot(pad_byte(j0)), gone_next;
     MaskWord mw[KT / 32] = {};
@@ -353,13 +376,15 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dq_ke
     }
     if (!live) return;
     const float back = static_cast<float>(p.scale) / ds_scale * (kScaled<T> ? 0x1p-15f : 1.f);
+    const int64_t part_at = ((static_cast<int64_t>(work.tile - parts.t.whole) * work.parts + work.part) * (WK ? 32 : 128) +
+                             r - row0) * p.D;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
             const int at = 32 * d + 8 * x + 4 * half;
-            if (parts.n > 1)
-                store4<float>(parts.a + split * parts.outputs + out_at, at, p.D, vec_out, dq[d], 4 * x, back);
+            if (work.parts > 1)
+                store4<float>(parts.a + part_at, at, p.D, p.D % 4 == 0, dq[d], 4 * x, back);
             else
                 store4<T>(static_cast<T*>(p.dq) + out_at, at, p.D, vec_out, dq[d], 4 * x, back);
         }
@@ -394,10 +419,9 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dkv_k
     constexpr int KW = WK ? 1 : 4;  // words of 32 keys that the workgroup's keys have
     constexpr int kArea = 2 * kTile + RT * dkv_row_bytes<WK, MASK>();
     extern __shared__ __align__(16) unsigned char lds[];
-    const int id = xcd_order(static_cast<int>(blockIdx.x), p.B * p.Hk * tiles * parts.n);
-    if (id < 0) return;
-    const int split = id % parts.n, tile = id / parts.n % tiles, bh = id / parts.n / tiles;  // causal: the first keys are
-                                                                                            // seen by the most rows
+    const TileWork work = tile_work(parts.t);
+    if (work.tile < 0) return;
+    const int tile = work.tile % tiles, bh = work.tile / tiles;  // causal: the first keys are seen by the most rows
     const int b = bh / p.Hk, hk = bh % p.Hk;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
     const int lane = threadIdx.x % kWave, half = lane >> 5;
@@ -511,9 +535,9 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dkv_k
 
     constexpr int step = WK ? 4 * RT : RT;
     int64_t rend = p.rows;
-    if (parts.n > 1) {
-        const int64_t each = (p.rows > r0 ? p.rows - r0 + parts.n * step - 1 : 0) / (parts.n * step) * step;
-        r0 += split * each;
+    if (work.parts > 1) {
+        const int64_t n = work.parts, each = (p.rows > r0 ? p.rows - r0 + n * step - 1 : 0) / (n * step) * step;
+        r0 += work.part * each;
         rend = r0 + each < rend ? r0 + each : rend;
     }
     if (WK) r0 += wave * RT;
@@ -647,15 +671,17 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dkv_k
     const float pv = live ? (kScaled<T> ? 0x1p-15f : 1.f) : 0.f;
     const float back = static_cast<float>(p.scale) / ds_scale * (kScaled<T> ? 0x1p-15f : 1.f);
     const int64_t at = ((static_cast<int64_t>(b) * p.K + j) * p.Hk + hk) * p.D;
+    const int64_t part_at = ((static_cast<int64_t>(work.tile - parts.t.whole) * work.parts + work.part) * (WK ? 32 : 128) +
+                             j - key0) * p.D;
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
         if (!live) dk[d] = dv[d] = f32x16{0.f};  // a key that nobody sees: its column may hold anything
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
             const int c = 32 * d + 8 * x + 4 * half;
-            if (parts.n > 1) {
-                store4<float>(parts.a + split * parts.outputs + at, c, p.D, vec_out, dk[d], 4 * x, back);
-                store4<float>(parts.b + split * parts.outputs + at, c, p.D, vec_out, dv[d], 4 * x, pv);
+            if (work.parts > 1) {
+                store4<float>(parts.a + part_at, c, p.D, p.D % 4 == 0, dk[d], 4 * x, back);
+                store4<float>(parts.b + part_at, c, p.D, p.D % 4 == 0, dv[d], 4 * x, pv);
             } else {
                 store4<T>(static_cast<T*>(p.dk) + at, c, p.D, vec_out, dk[d], 4 * x, back);
                 store4<T>(static_cast<T*>(p.dv) + at, c, p.D, vec_out, dv[d], 4 * x, pv);
@@ -665,8 +691,14 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dkv_k
 }
 
 struct BackShape {
-    bool vec, wk_q, wk_k;
-    int q_tiles, k_tiles, q_parts, k_parts;
+    bool vec;
+    struct One {
+        bool wk;
+        int tiles;
+        TileSplit t;
+        int tile_rows() const { return wk ? 32 : 128; }
+        int64_t part_floats(int D) const { return static_cast<int64_t>(t.total - t.whole) * t.n * tile_rows() * D; }
+    } q, k;
 };
 
 bool back_vec(int dtype, const AttnParams& p) {
@@ -683,24 +715,30 @@ bool back_vec(int dtype, const AttnParams& p) {
 
 // Workgroups of 128 rows (keys) that share tiles, when they fill the GPU twice; else of 32 rows (keys) with the others'
 // tiles over the wavefronts, which needs no second launch, for heads whose private tiles fit in the registers. Where that
-// still leaves CUs without work and the loops are long, parts.
+// still leaves CUs without work and the loops are long, parts; where many tiles leave a few over, parts of those
+// (even_split).
 BackShape back_shape(int dtype, const AttnParams& p, bool vec) {
     BackShape s{};
     s.vec = vec;
     const int64_t heads = static_cast<int64_t>(p.B) * p.Hk;
     const bool can = vec && padded_width(p.D) * elem_size(dtype) <= 128;
-    auto shape = [&](int n, int over, bool& wk, int& tiles, int& parts) {
-        wk = can && heads * ((n + 127) / 128) < 512;
-        tiles = wk ? (n + 31) / 32 : (n + 127) / 128;
-        parts = 1;
-        const int64_t groups = heads * tiles;
-        if (groups == 0 || groups >= 384) return;
-        const int64_t want = (1024 + groups - 1) / groups, most = over / 512;  // 4 steps of 4 x 32 or 16 of 32 a part
-        parts = static_cast<int>(want < most ? want : most);
-        parts = parts < 1 ? 1 : parts;
+    auto shape = [&](int n, int over) {
+        BackShape::One o{};
+        o.wk = can && heads * ((n + 127) / 128) < 512;
+        o.tiles = o.wk ? (n + 31) / 32 : (n + 127) / 128;
+        const int total = static_cast<int>(heads * o.tiles);
+        o.t = TileSplit{1, total, total};
+        if (total > 0 && total < 384) {
+            const int want = (1024 + total - 1) / total, most = over / 512;  // 4 steps of 4 x 32 or 16 of 32 a part
+            const int parts = want < most ? want : most;
+            if (parts > 1) o.t = TileSplit{parts, 0, total};
+        } else if (!o.wk && !p.causal) {
+            o.t = even_split(total, (over + 63) / 64);
+        }
+        return o;
     };
-    shape(p.rows, p.K, s.wk_q, s.q_tiles, s.q_parts);
-    shape(p.K, p.rows, s.wk_k, s.k_tiles, s.k_parts);
+    s.q = shape(p.rows, p.K);
+    s.k = shape(p.K, p.rows);
     return s;
 }
 
@@ -716,10 +754,9 @@ int run_dq(const AttnParams& p, const BackShape& s, const RowInfo& info, float* 
         bytes > 64 * 1024 ? allow_dynamic_lds(reinterpret_cast<const void*>(fn), bytes, done) : hipSuccess;
     if (e != hipSuccess) return set_error(TD_E_LAUNCH, "attention backward: LDS size: %s", hipGetErrorString(e));
     const bool vec_out = p.D % 4 == 0 && reinterpret_cast<uintptr_t>(p.dq) % (4 * sizeof(T)) == 0;
-    const Parts parts{s.q_parts, ws, nullptr, static_cast<int64_t>(p.B) * p.Q * p.H * p.D};
-    const int64_t n = static_cast<int64_t>(p.B) * p.Hk * s.q_tiles * parts.n;
-    hipLaunchKernelGGL(fn, dim3(xcd_grid(n)), dim3(256), bytes, stream, p, info, parts, vec_out, s.q_tiles);
-    if (parts.n > 1) sum_parts<T>(parts.a, parts, p.dq, stream);
+    const Parts parts{s.q.t, ws, nullptr};
+    hipLaunchKernelGGL(fn, dim3(tile_grid(s.q.t)), dim3(256), bytes, stream, p, info, parts, vec_out, s.q.tiles);
+    if (s.q.t.n > 1) sum_parts<T>(p, s.q.t, parts.a, p.dq, s.q.tile_rows(), s.q.tiles, false, stream);
     return 0;
 }
 
@@ -737,13 +774,11 @@ int run_dkv(const AttnParams& p, const BackShape& s, const RowInfo& info, float*
     if (e != hipSuccess) return set_error(TD_E_LAUNCH, "attention backward: LDS size: %s", hipGetErrorString(e));
     const bool vec_out = p.D % 4 == 0 && reinterpret_cast<uintptr_t>(p.dk) % (4 * sizeof(T)) == 0 &&
                          reinterpret_cast<uintptr_t>(p.dv) % (4 * sizeof(T)) == 0;
-    const int64_t outputs = static_cast<int64_t>(p.B) * p.K * p.Hk * p.D;
-    const Parts parts{s.k_parts, ws, ws + s.k_parts * outputs, outputs};
-    const int64_t n = static_cast<int64_t>(p.B) * p.Hk * s.k_tiles * parts.n;
-    hipLaunchKernelGGL(fn, dim3(xcd_grid(n)), dim3(256), bytes, stream, p, info, parts, vec_out, s.k_tiles);
-    if (parts.n > 1) {
-        sum_parts<T>(parts.a, parts, p.dk, stream);
-        sum_parts<T>(parts.b, parts, p.dv, stream);
+    const Parts parts{s.k.t, ws, ws + s.k.part_floats(p.D)};
+    hipLaunchKernelGGL(fn, dim3(tile_grid(s.k.t)), dim3(256), bytes, stream, p, info, parts, vec_out, s.k.tiles);
+    if (s.k.t.n > 1) {
+        sum_parts<T>(p, s.k.t, parts.a, p.dk, s.k.tile_rows(), s.k.tiles, true, stream);
+        sum_parts<T>(p, s.k.t, parts.b, p.dv, s.k.tile_rows(), s.k.tiles, true, stream);
     }
     return 0;
 }
@@ -756,7 +791,7 @@ int run_dp(const AttnParams& p, const BackShape& s, const RowInfo& info, float* 
         if (!s.vec)
             rc = mask ? run_dq<T, DP, false, true, false>(p, s, info, ws, stream)
                       : run_dq<T, DP, false, false, false>(p, s, info, ws, stream);
-        else if (!s.wk_q)
+        else if (!s.q.wk)
             rc = mask ? run_dq<T, DP, false, true, true>(p, s, info, ws, stream)
                       : run_dq<T, DP, false, false, true>(p, s, info, ws, stream);
         else if constexpr (DP * sizeof(T) <= 128)
@@ -767,7 +802,7 @@ int run_dp(const AttnParams& p, const BackShape& s, const RowInfo& info, float* 
         if (!s.vec)
             rc = mask ? run_dkv<T, DP, false, true, false>(p, s, info, ws, stream)
                       : run_dkv<T, DP, false, false, false>(p, s, info, ws, stream);
-        else if (!s.wk_k)
+        else if (!s.k.wk)
             rc = mask ? run_dkv<T, DP, false, true, true>(p, s, info, ws, stream)
                       : run_dkv<T, DP, false, false, true>(p, s, info, ws, stream);
         else if constexpr (DP * sizeof(T) <= 128)
@@ -828,8 +863,7 @@ int64_t attn_backward_workspace(int dtype, const AttnParams& p) {
     int64_t parts = 0;  // dQ's and then dK's and dV's
     for (const bool vec : {false, true}) {  // the gradients' alignment is not known yet
         const BackShape s = back_shape(dtype, p, vec);
-        const int64_t q = s.q_parts > 1 ? static_cast<int64_t>(s.q_parts) * p.B * p.Q * p.H * p.D : 0;
-        const int64_t k = s.k_parts > 1 ? 2 * static_cast<int64_t>(s.k_parts) * p.B * p.K * p.Hk * p.D : 0;
+        const int64_t q = s.q.part_floats(p.D), k = 2 * s.k.part_floats(p.D);
         parts = parts > q ? parts : q;
         parts = parts > k ? parts : k;
     }

@@ -23,10 +23,10 @@ template <typename T>
 constexpr float kShift = std::is_same<T, f16>::value ? 11.f : 0.f;
 
 struct Split {
-    int n;      // key ranges a row's keys are split over (1: none)
-    int keys;   // keys of a range, a multiple of 64
-    float* o;   // [n][B * H * Q][D] unnormalised outputs
-    float* ml;  // [n][B * H * Q][2] maximum and sum
+    TileSplit t;
+    int keys;   // keys of a part, a multiple of 256
+    float* o;   // parts' unnormalised outputs [..][rows of a tile][D]
+    float* ml;  // and maximum and sum [..][rows of a tile][2]
 };
 
 // Keys of a tile: 64 where the staged rows leave room for two workgroups on a CU
@@ -43,6 +43,15 @@ constexpr int min_waves() {
     return n > 1 && bytes <= 128 && (WK || SLOW) ? n - 1 : SLOW ? 1 : n;
 }
 
+// 16-bit rows of up to 64 elements: the kernel is bound by the vector units (a score takes a fused multiply-add, an
+// exponential at a quarter of the rate, half a maximum, half a conversion and an addition: 28 cycles of a SIMD, its share
+// of the products 8 or 16), and l is summed by the matrix units, as one more column of ones of V. It is then the sum of
+// the rounded probabilities, which is also what O is a sum of.
+template <typename T, int DP, bool WK>
+constexpr bool sum_by_mma() {
+    return sizeof(T) == 2 && DP <= 64 && !WK;
+}
+
 // WK false: four wavefronts of 32 rows each share the key tiles of the workgroup's 128 rows. WK true: the workgroup has
 // 32 rows and each wavefront every fourth key tile, in LDS of its own; the four partial results are joined in LDS.
 // MASK: there is a mask tensor. VEC: operands are read 16 bytes at a time (StagedRows).
@@ -53,9 +62,9 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
     constexpr int KT = key_tile<T, DP, WK>(), NT = WK ? 64 : 256, ND = DP / 32;
     constexpr int kTile = KT * R::kPitch;
     extern __shared__ __align__(16) unsigned char lds[];
-    const int id = xcd_order(static_cast<int>(blockIdx.x), p.B * p.Hk * tiles * sp.n);
-    if (id < 0) return;
-    const int split = id % sp.n, tile = tiles - 1 - id / sp.n % tiles, bh = id / sp.n / tiles;  // causal: long ones first
+    const TileWork work = tile_work(sp.t);
+    if (work.tile < 0) return;
+    const int tile = tiles - 1 - work.tile % tiles, bh = work.tile / tiles;  // causal: the long ones first
     const int b = bh / p.Hk, hk = bh % p.Hk;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
     const int lane = threadIdx.x % kWave, half = lane >> 5;
@@ -86,8 +95,8 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
         const int seen = static_cast<int>(fast_div(p.gdiv, static_cast<uint32_t>(top_row))) + diag + 1;
         kend = seen < kend ? seen : kend;
     }
-    if (sp.n > 1) {
-        k0 = split * sp.keys;
+    if (work.parts > 1) {
+        k0 = work.part * sp.keys;
         kend = k0 + static_cast<int64_t>(sp.keys) < kend ? k0 + sp.keys : kend;
     }
     const int wtop = wrow0 + 31 < p.rows ? wrow0 + 31 : p.rows - 1;
@@ -110,9 +119,15 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
     ks.plan(k_row, p.D, t);
     vs.plan(v_row, p.D, t);
     float m = kNegInf, l = 0.f;
-    f32x16 o[ND];
+    f32x16 o[ND], lm = f32x16{0.f};
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = f32x16{0.f};
+    constexpr bool kSumMma = sum_by_mma<T, DP, WK>();
+    u32x4 ones = {0u, 0u, 0u, 0u};
+    if constexpr (kSumMma) {
+        const unsigned short one = __builtin_bit_cast(unsigned short, static_cast<T>(1.f));
+        ones = u32x4{1u, 1u, 1u, 1u} * (one * 0x10001u);
+    }
 
     constexpr int step = WK ? 4 * KT : KT;
     constexpr uint64_t all = KT == 64 ? ~uint64_t{0} : (uint64_t{1} << (KT & 63)) - 1;
@@ -182,7 +197,10 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
                 const float to = __builtin_fmaxf(m, mt);
                 const float shrink = to == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m - to);
                 m = to;
-                l *= shrink;
+                if constexpr (kSumMma)
+                    lm *= shrink;
+                else
+                    l *= shrink;
 #pragma unroll
                 for (int d = 0; d < ND; ++d) o[d] *= shrink;
             }
@@ -193,10 +211,13 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     pr[e] = __builtin_amdgcn_exp2f(fmaf(s[x][e], cc, -from));
-                    l += pr[e];
+                    if constexpr (!kSumMma) l += pr[e];
                 }
                 typename R::Packed w[R::kPacked];
                 R::pack(pr, w);
+                if constexpr (kSumMma)
+#pragma unroll
+                    for (int y = 0; y < R::kPacked; ++y) lm = Mma<T>::mul(ones, w[y], lm);
 #pragma unroll
                 for (int d = 0; d < ND; ++d) o[d] = R::columns(vt_lds, 32 * x, 32 * d, lane, w, o[d]);
             }
@@ -204,7 +225,7 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
         gone = gone_next;
         if (WK) wave_sync();
     }
-    l += other_half(l);
+    l = kSumMma ? lm[0] : l + other_half(l);
 
     if constexpr (WK) {
         // join the four wavefronts' parts: maxima and sums first, then each scaled O, through LDS
@@ -260,16 +281,14 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
     if (!live) return;
 
     const int64_t row = (static_cast<int64_t>(b) * p.H + h) * p.Q + i;
-    if (sp.n > 1) {
-        const int64_t part = static_cast<int64_t>(split) * p.B * p.H * p.Q + row;
-        float* const to = sp.o + part * p.D;
+    if (work.parts > 1) {
+        const int64_t part = (static_cast<int64_t>(work.tile - sp.t.whole) * work.parts + work.part) * (WK ? 32 : 128) +
+                             (r - row0);
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int at = 32 * d + 8 * (e >> 2) + 4 * half + (e & 3);
-                if (at < p.D) to[at] = o[d][e];
-            }
+            for (int x = 0; x < 4; ++x)
+                store4<float>(sp.o + part * p.D, 32 * d + 8 * x + 4 * half, p.D, p.D % 4 == 0, o[d], 4 * x, 1.f);
         if (half == 0) {
             sp.ml[2 * part] = m;
             sp.ml[2 * part + 1] = l;
@@ -299,66 +318,87 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
     }
 }
 
-// Joins the key ranges of each row: a workgroup a row. The ranges' factors 2^(m_s - m) / l go to LDS first, then 256 / W
-// groups of W threads, W the channels rounded up to a power of two, each add every group's share of the ranges.
-constexpr int kJoinRanges = 1024;  // most ranges of a row (shape_of)
+// Joins the parts of each row: out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s. A row has 256 / rows threads of the
+// workgroup: with many parts all of them (a decoded token over a long cache has few rows and hundreds of parts), which
+// each add every fourth or so part of a channel; with a few parts one for each channel.
+constexpr int kJoinParts = 1024;  // most parts of a row (shape_of)
 template <typename T>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p, Split sp, int wide) {
-    __shared__ float factor[kJoinRanges], part[256], best[4], total[4];
-    const int t = threadIdx.x, lane = t % kWave, wave = t / kWave;
-    const int64_t row = blockIdx.x, rows = static_cast<int64_t>(p.B) * p.H * p.Q;
-    float m = kNegInf;
-    for (int s = t; s < sp.n; s += 256) m = __builtin_fmaxf(m, sp.ml[2 * (s * rows + row)]);
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p, Split sp, int wide, int rows, int tile_rows,
+                                                        int tiles) {
+    __shared__ float factor[kJoinParts], part[256];
+    const int t = threadIdx.x, each = 256 / rows, x = t % each, n = sp.t.n;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * rows + t / each;  // row of a tile that is split
+    const int left = static_cast<int>(at / tile_rows), row = static_cast<int>(at % tile_rows);
+    const int tile = sp.t.whole + left, bh = tile / tiles, r = (tiles - 1 - tile % tiles) * tile_rows + row;
+    const bool live = r < p.rows;
+    if (rows == 1 && !live) return;
+    const int64_t part0 = (static_cast<int64_t>(left) * n) * tile_rows + row;  // part s: + s * tile_rows
+    const int b = bh / p.Hk, i = static_cast<int>(fast_div(p.gdiv, static_cast<uint32_t>(live ? r : 0)));
+    const int h = bh % p.Hk * p.G + (live ? r : 0) - i * p.G;
+    float m = kNegInf, l = 0.f, o = 0.f;
+    const int d = x % wide, group = x / wide, groups = each / wide;
+    if (rows == 1) {
+        for (int s = t; s < n; s += 256) m = __builtin_fmaxf(m, sp.ml[2 * (part0 + static_cast<int64_t>(s) * tile_rows)]);
 #pragma unroll
-    for (int x = 32; x > 0; x >>= 1) m = __builtin_fmaxf(m, xor_lane(m, x));
-    if (lane == 0) best[wave] = m;
-    __syncthreads();
-    m = __builtin_fmaxf(__builtin_fmaxf(best[0], best[1]), __builtin_fmaxf(best[2], best[3]));
-    float l = 0.f;
-    for (int s = t; s < sp.n; s += 256) {
-        const float* ml = sp.ml + 2 * (s * rows + row);
-        const float f = ml[0] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(ml[0] - m);
-        factor[s] = f;
-        l = fmaf(ml[1], f, l);
-    }
-    l = wave_sum(l);
-    if (lane == 0) total[wave] = l;
-    __syncthreads();
-    l = (total[0] + total[1]) + (total[2] + total[3]);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int64_t i = row % p.Q, h = row / p.Q % p.H, b = row / p.Q / p.H;
-    const int64_t out_at = ((b * p.Q + i) * p.H + h) * p.D;
-    const int d = t % wide, group = t / wide, groups = 256 / wide;
-    float o = 0.f;
-    if (d < p.D) {
+        for (int y = 32; y > 0; y >>= 1) m = __builtin_fmaxf(m, xor_lane(m, y));
+        if (t % kWave == 0) part[t / kWave] = m;
+        __syncthreads();
+        m = __builtin_fmaxf(__builtin_fmaxf(part[0], part[1]), __builtin_fmaxf(part[2], part[3]));
+        for (int s = t; s < n; s += 256) {
+            const float* ml = sp.ml + 2 * (part0 + static_cast<int64_t>(s) * tile_rows);
+            const float f = ml[0] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(ml[0] - m);
+            factor[s] = f;
+            l = fmaf(ml[1], f, l);
+        }
+        l = wave_sum(l);
+        if (t % kWave == 0) part[4 + t / kWave] = l;
+        __syncthreads();
+        l = (part[4] + part[5]) + (part[6] + part[7]);
+        if (d < p.D) {
 #pragma unroll 4
-        for (int s = group; s < sp.n; s += groups) {
-            const float f = factor[s];
-            if (f != 0.f) o = fmaf(sp.o[(s * rows + row) * p.D + d], f, o);
+            for (int s = group; s < n; s += groups) {
+                const float f = factor[s];
+                if (f != 0.f) o = fmaf(sp.o[(part0 + static_cast<int64_t>(s) * tile_rows) * p.D + d], f, o);
+            }
+        }
+        __syncthreads();
+        part[t] = o;
+        __syncthreads();
+        if (group == 0)
+            for (int g = 1; g < groups; ++g) o += part[g * wide + d];
+    } else if (live) {
+        for (int s = 0; s < n; ++s) m = __builtin_fmaxf(m, sp.ml[2 * (part0 + static_cast<int64_t>(s) * tile_rows)]);
+        for (int s = 0; s < n; ++s) {
+            const int64_t q = part0 + static_cast<int64_t>(s) * tile_rows;
+            const float f = sp.ml[2 * q] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(sp.ml[2 * q] - m);
+            l = fmaf(sp.ml[2 * q + 1], f, l);
+            if (f != 0.f && d < p.D) o = fmaf(sp.o[q * p.D + d], f, o);
         }
     }
-    part[t] = o;
-    __syncthreads();
-    if (group == 0 && d < p.D) {
-        for (int g = 1; g < groups; ++g) o += part[g * wide + d];
-        o *= inv;
+    if (!live || group != 0) return;
+    if (d < p.D) {
+        const int64_t out_at = ((static_cast<int64_t>(b) * p.Q + i) * p.H + h) * p.D + d;
+        o *= l == 0.f ? 0.f : 1.f / l;
         const T v = static_cast<T>(o);
-        static_cast<T*>(p.out)[out_at + d] = v;
+        static_cast<T*>(p.out)[out_at] = v;
         if (sizeof(T) == 2 && p.out_low != nullptr)
-            static_cast<T*>(p.out_low)[out_at + d] = static_cast<T>(o - static_cast<float>(v));
+            static_cast<T*>(p.out_low)[out_at] = static_cast<T>(o - static_cast<float>(v));
     }
-    if (p.stats != nullptr && t == 0) {
-        float* const st = static_cast<float*>(p.stats) + 2 * row;
+    if (p.stats != nullptr && x == 0) {
+        float* const st = static_cast<float*>(p.stats) + 2 * ((static_cast<int64_t>(b) * p.H + h) * p.Q + i);
         st[0] = l == 0.f ? 0.f : m;
         st[1] = l == 0.f ? 0.f : __builtin_amdgcn_logf(l) - kShift<T>;
     }
 }
 
-// The launch shape. Workgroups of 128 rows that share key tiles, when they fill the GPU twice; else workgroups of 32 rows
-// with the keys over the wavefronts, and when those are few and the keys many, the keys over several workgroups too.
+// The launch shape. Workgroups of 128 rows that share key tiles, when they fill the GPU twice, with what is left over after
+// an even share for every CU split (even_split); else workgroups of 32 rows with the keys over the wavefronts, and when
+// those are few and the keys many, the keys over several workgroups too.
 struct Shape {
     bool vec, wk;
-    int tiles, n, keys;
+    int tiles, keys;
+    TileSplit t;
+    int tile_rows() const { return wk ? 32 : 128; }
 };
 
 Shape shape_of(int dtype, const AttnParams& p) {
@@ -373,19 +413,25 @@ Shape shape_of(int dtype, const AttnParams& p) {
     const bool can = s.vec && padded_width(p.D) * elem <= 256;  // wider rows' private tiles do not fit in registers
     s.wk = can && heads * ((p.rows + 127) / 128) < 512;
     s.tiles = s.wk ? (p.rows + 31) / 32 : (p.rows + 127) / 128;
-    s.n = 1;
-    s.keys = p.K;
-    const int64_t groups = heads * s.tiles;
-    if (groups < 512 && p.K > 1024) {
-        int64_t n = (1024 + groups - 1) / groups;
+    const int total = static_cast<int>(heads * s.tiles);
+    s.t = TileSplit{1, total, total};
+    if (total < 512 && p.K > 1024) {
+        int64_t n = (1024 + total - 1) / total;
         const int64_t most = (p.K + 511) / 512;
         n = n < most ? n : most;
-        n = n < kJoinRanges ? n : kJoinRanges;
-        const int64_t keys = ((p.K + n - 1) / n + 255) / 256 * 256;
-        s.keys = static_cast<int>(keys);
-        s.n = static_cast<int>((p.K + keys - 1) / keys);
+        n = n < kJoinParts ? n : kJoinParts;
+        s.t = TileSplit{static_cast<int>(n), n > 1 ? 0 : total, total};
+    } else if (!s.wk && !p.causal) {  // causal tiles differ in length and even out by themselves
+        s.t = even_split(total, (p.K + 63) / 64);
     }
+    const int64_t keys = ((p.K + s.t.n - 1) / s.t.n + 255) / 256 * 256;
+    s.keys = static_cast<int>(keys < 2147483392 ? keys : 2147483392);
     return s;
+}
+
+// Floats that the parts take: their outputs, maxima and sums
+int64_t part_floats(const AttnParams& p, const Shape& s) {
+    return static_cast<int64_t>(s.t.total - s.t.whole) * s.t.n * s.tile_rows() * (p.D + 2);
 }
 
 template <typename T, int DP, bool WK, bool MASK, bool VEC>
@@ -399,13 +445,15 @@ int run(const AttnParams& p, const Shape& s, const Split& sp, hipStream_t stream
     const hipError_t e =
         bytes > 64 * 1024 ? allow_dynamic_lds(reinterpret_cast<const void*>(fn), bytes, done) : hipSuccess;
     if (e != hipSuccess) return set_error(TD_E_LAUNCH, "attention: LDS size: %s", hipGetErrorString(e));
-    const int64_t n = static_cast<int64_t>(p.B) * p.Hk * s.tiles * s.n;
     const bool vec_out = p.D % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.out_low)) %
                                                  (4 * sizeof(T)) == 0;
-    hipLaunchKernelGGL(fn, dim3(xcd_grid(n)), dim3(256), bytes, stream, p, sp, vec_out, s.tiles);
-    if (s.n > 1)
-        hipLaunchKernelGGL((attn_join_kernel<T>), dim3(static_cast<unsigned>(p.B) * p.H * p.Q), dim3(256), 0, stream, p,
-                           sp, padded_width(p.D));
+    hipLaunchKernelGGL(fn, dim3(tile_grid(sp.t)), dim3(256), bytes, stream, p, sp, vec_out, s.tiles);
+    if (sp.t.n > 1) {
+        const int rows = sp.t.n <= 16 ? 256 / padded_width(p.D) : 1;  // of a workgroup; a tile's are a multiple of it
+        const int64_t groups = static_cast<int64_t>(sp.t.total - sp.t.whole) * s.tile_rows() / rows;
+        hipLaunchKernelGGL((attn_join_kernel<T>), dim3(static_cast<unsigned>(groups)), dim3(256), 0, stream, p, sp,
+                           padded_width(p.D), rows, s.tile_rows(), s.tiles);
+    }
     const hipError_t le = hipGetLastError();
     return le == hipSuccess ? 0 : set_error(TD_E_LAUNCH, "attention launch failed: %s", hipGetErrorString(le));
 }
@@ -429,10 +477,9 @@ int run_dp(const AttnParams& p, const Shape& s, const Split& sp, hipStream_t str
 template <typename T>
 int launch_attn_forward_t(int dtype, const AttnParams& p, hipStream_t stream) {
     const Shape s = shape_of(dtype, p);
-    const int64_t rows = static_cast<int64_t>(p.B) * p.H * p.Q;
     AttnParams q = p;
     float* const ws = reinterpret_cast<float*>(static_cast<unsigned char*>(p.ws) + plan_mask(q, p.ws));
-    const Split sp{s.n, s.keys, ws, ws + s.n * rows * p.D};
+    const Split sp{s.t, s.keys, ws, ws + part_floats(p, s) / (p.D + 2) * p.D};
     const int rc = launch_mask(dtype, q, stream);
     if (rc != 0) return rc;
     switch (padded_width(p.D)) {
@@ -450,7 +497,7 @@ int64_t attn_forward_workspace(int dtype, const AttnParams& p) {
     if (dtype == kF64) return 0;
     const Shape s = shape_of(dtype, p);
     AttnParams q = p;
-    return plan_mask(q, nullptr) + (s.n == 1 ? 0 : static_cast<int64_t>(s.n) * p.B * p.H * p.Q * (p.D + 2) * 4);
+    return plan_mask(q, nullptr) + part_floats(p, s) * 4;
 }
 
 int launch_attn_forward(int dtype, const AttnParams& p, hipStream_t stream) {

@@ -206,6 +206,39 @@ __device__ __forceinline__ int xcd_order(int w, int n) {
 }
 inline unsigned xcd_grid(int64_t n) { return static_cast<unsigned>((n + kXcds - 1) / kXcds * kXcds); }
 
+// Work that is split: tiles (of rows or keys, numbered over the batch and key heads) before `whole` have a workgroup each,
+// those from it on n, which write float32 parts [tile - whole][part][rows of a tile][D] that are joined afterwards.
+struct TileSplit {
+    int n, whole, total;
+};
+struct TileWork {
+    int tile, part, parts;  // tile < 0: no work
+};
+__device__ __forceinline__ TileWork tile_work(const TileSplit& s) {
+    const int block = static_cast<int>(blockIdx.x), first = (s.whole + kXcds - 1) / kXcds * kXcds;
+    if (block < first) return TileWork{xcd_order(block, s.whole), 0, 1};
+    const int i = xcd_order(block - first, (s.total - s.whole) * s.n);
+    return i < 0 ? TileWork{-1, 0, 1} : TileWork{s.whole + i / s.n, i % s.n, s.n};
+}
+inline unsigned tile_grid(const TileSplit& s) {
+    return xcd_grid(s.whole) + (s.n > 1 ? xcd_grid(static_cast<int64_t>(s.total - s.whole) * s.n) : 0);
+}
+// Every CU works at its own rate whether it holds four workgroups or one, so 4 1/8 tiles a CU take as long as 5. Where a
+// few tiles are left over after an even share for every CU, those are split over all CUs (8400 tokens of 16 heads are
+// 1056 tiles on 256 CUs: 322 us with the 32 left over whole, ... split).
+inline TileSplit even_split(int total, int steps) {
+    const int cus = cu_count(), rest = total % cus;
+    TileSplit s{1, total, total};
+    if (total < 2 * cus || total > 8 * cus || rest == 0 || rest > cus / 2) return s;
+    int n = cus / rest;
+    n = n < 8 ? n : 8;
+    n = n < steps / 4 ? n : steps / 4;
+    if (n < 2) return s;
+    s.n = n;
+    s.whole = total - rest;
+    return s;
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kLowest = -3.4028234663852886e38f;

@@ -98,6 +98,25 @@ def test_float64(mask):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
+def test_tiles_left_over_after_an_even_share(dtype):
+    # 130 heads of four tiles: on 256 CUs 512 tiles and 8 more, which several workgroups share. Heads at both ends
+    # against the oracle; the others are the first head's, bit for bit
+    one, two = (make_attn((1, 500, 500, 1, 1, 32), dtype, seed=i) for i in (0, 1))
+    for mask in (None, torch.rand(500, 500, generator=torch.Generator().manual_seed(2)) < 0.3):
+        kw = {} if mask is None else dict(attn_mask=mask)
+        q, k, v, go = (torch.cat([a.unflatten(-1, (-1, 32)) if a.dim() == 3 else a] * 129
+                                 + [b.unflatten(-1, (-1, 32)) if b.dim() == 3 else b], 2)
+                       for a, b in zip(one[:4], two[:4]))
+        out, grads = run(q, k, v, go.flatten(2), kw)
+        parts = [out.unflatten(-1, (130, 32))] + list(grads)
+        for h, (a, b, c, g, _) in ((0, one), (128, one), (129, two)):
+            at = [t[:, :, h:h + 1] for t in parts]
+            check_attn(dtype, a, b, c, g, kw, at[0].flatten(2), at[1:])
+        for t in parts:
+            assert torch.equal(t[:, :, :1].expand(-1, -1, 128, -1), t[:, :, :128])
+
+
+@pytest.mark.parametrize('dtype', TYPES)
 def test_a_row_left_nothing_gives_zeros(dtype):
     q, k, v, go, _ = make_attn((2, 40, 50, 2, 2, 32), dtype)
     mask = torch.zeros(2, 1, 40, 50, dtype=torch.bool)
