@@ -249,9 +249,11 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dq_ke
     const T* const kb = static_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[2];
     const T* const vb = static_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[2];
     const uint8_t* const pad = p.pad == nullptr ? nullptr : p.pad + static_cast<int64_t>(b) * p.K;
-    auto pad_byte = [&](int64_t j0) -> int {
+    auto pad_byte = [&](int64_t j0) {  // not looked at before the next tile: that would wait for the loads issued before it
         const int64_t j = j0 + lane;
-        return lane >= KT || j >= kend || (pad != nullptr && pad[j] != 0);
+        int v = 1;
+        if (lane < KT && j < kend) v = pad != nullptr ? pad[j] : 0;
+        return v;
     };
     StagedRows<T, DP, KT, NT, VEC> ks, vs;
     auto k_row = [&](int x) { return x * p.ks[1]; };
@@ -270,7 +272,7 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dq_ke
         j0 += work.part * each;
         kend = (work.part + 1) * each < kend ? static_cast<int>((work.part + 1) * each) : kend;
     }
-    uint64_t gone = __ballot(pad_byte(j0)), gone_next;
+    uint64_t gone = __ballot(pad_byte(j0) != 0), gone_next;
     MaskWord mw[KT / 32] = {};
     auto fetch = [&](int64_t at, uint64_t g) {
         if constexpr (MASK)
@@ -283,13 +285,13 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dq_ke
     int next_pad = pad_byte(j0 + step);
     for (; j0 < kend; j0 += step) {
         if (!WK) __syncthreads();
-        ks.store(kt_lds, t);
-        vs.store(vt_lds, t);
+        ks.store(kt_lds, p.D, t);
+        vs.store(vt_lds, p.D, t);
         if (WK)
             wave_sync();
         else
             __syncthreads();
-        gone_next = __ballot(next_pad);
+        gone_next = __ballot(next_pad != 0);
         uint32_t bits[KT / 32];
         bool masked[KT / 32], values[KT / 32], none[KT / 32];
 #pragma unroll
@@ -498,8 +500,9 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dkv_k
     }
     f32x4 ri = f32x4{0.f, 0.f, 0.f, 0.f};
     int64_t mo = 0;
-    uint32_t words[KW] = {};
-    int kinds[KW] = {};
+    MaskWord words[KW] = {};
+    bool in_rows = false;
+    int sees = 0;  // the last key that the row sees
     const bool bits = MASK || p.causal;
     auto fetch = [&](int64_t at) {
         from_row = at;
@@ -513,19 +516,16 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dkv_k
         qs.load(qb + i0 * p.qs[1], q_row, gone, p.D, t);
         gs.load(gb + i0 * gs1, g_row, gone, p.D, t);
         if (t < RT) {
-            const bool in = t < left;
+            const bool in = in_rows = t < left;
             ri = in ? ib[at + t] : f32x4{__builtin_inff(), 0.f, 0.f, 0.f};
             if (bits) {
                 const int i = static_cast<int>(fast_div(p.gdiv, static_cast<uint32_t>(in ? at + t : 0)));
                 const int h = hk * p.G + static_cast<int>(in ? at + t : 0) - i * p.G;
                 if (MASK) mo = b * p.ms[0] + h * p.ms[1] + i * p.ms[2];
+                sees = p.causal ? i + diag : 2147483647;
+                if (MASK)
 #pragma unroll
-                for (int w = 0; w < KW; ++w) {
-                    MaskWord m{0u, kMaskNone};
-                    if (MASK) m = mask_word(p, b, h, i, key0 / 32 + w);
-                    words[w] = m.bits | (p.causal ? beyond(key0 + 32 * w, i + diag) : 0u);
-                    kinds[w] = in ? m.kind : kMaskAll;
-                }
+                    for (int w = 0; w < KW; ++w) words[w] = mask_word(p, b, h, i, key0 / 32 + w);
             }
         }
     };
@@ -544,8 +544,8 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dkv_k
     if (r0 < rend) fetch(r0);
     for (; r0 < rend; r0 += step) {
         if (!WK) __syncthreads();
-        qs.store(q_lds, t);
-        gs.store(g_lds, t);
+        qs.store(q_lds, p.D, t);
+        gs.store(g_lds, p.D, t);
         if (t < RT) {
             m_lds[t] = apart ? ri[0] : ri[0] + ri[1] - kPShift<T>;
             l_lds[t] = ri[1] - kPShift<T>;
@@ -554,8 +554,8 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dkv_k
             if (bits) {
 #pragma unroll
                 for (int w = 0; w < KW; ++w) {
-                    w_lds[w * RT + t] = words[w];
-                    if (MASK) k_lds[w * RT + t] = kinds[w];
+                    w_lds[w * RT + t] = words[w].bits | beyond(key0 + 32 * w, sees);
+                    if (MASK) k_lds[w * RT + t] = in_rows ? words[w].kind : kMaskAll;
                 }
             }
         }
@@ -856,6 +856,8 @@ int launch_attn_backward_t(int dtype, const AttnParams& given, hipStream_t strea
 }
 
 #if TD_ATTN_TYPE == 0
+extern template int launch_attn_backward_t<f16>(int, const AttnParams&, hipStream_t);
+extern template int launch_attn_backward_t<bf16>(int, const AttnParams&, hipStream_t);
 template int launch_attn_backward_t<float>(int, const AttnParams&, hipStream_t);
 
 int64_t attn_backward_workspace(int dtype, const AttnParams& p) {

@@ -108,9 +108,11 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
     const T* const vb = static_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[2];
     const uint8_t* const pad = p.pad == nullptr ? nullptr : p.pad + static_cast<int64_t>(b) * p.K;
     // keys j0 + lane of a tile: whether nobody sees them
-    auto pad_byte = [&](int64_t j0) -> int {
+    auto pad_byte = [&](int64_t j0) {  // not looked at before the next tile: that would wait for the loads issued before it
         const int64_t j = j0 + lane;
-        return lane >= KT || j >= kend || (pad != nullptr && pad[j] != 0);
+        int v = 1;
+        if (lane < KT && j < kend) v = pad != nullptr ? pad[j] : 0;
+        return v;
     };
 
     StagedRows<T, DP, KT, NT, VEC> ks, vs;
@@ -132,7 +134,7 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
     constexpr int step = WK ? 4 * KT : KT;
     constexpr uint64_t all = KT == 64 ? ~uint64_t{0} : (uint64_t{1} << (KT & 63)) - 1;
     int64_t j0 = k0 + (WK ? wave * KT : 0);
-    uint64_t gone = __ballot(pad_byte(j0)), gone_next;
+    uint64_t gone = __ballot(pad_byte(j0) != 0), gone_next;
     MaskWord mw[KT / 32] = {};
     auto fetch = [&](int64_t at, uint64_t g) {
         if constexpr (MASK)
@@ -145,13 +147,13 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
     int next_pad = pad_byte(j0 + step);
     for (; j0 < kend; j0 += step) {
         if (!WK) __syncthreads();
-        ks.store(kt_lds, t);
-        vs.store(vt_lds, t);
+        ks.store(kt_lds, p.D, t);
+        vs.store(vt_lds, p.D, t);
         if (WK)
             wave_sync();
         else
             __syncthreads();
-        gone_next = __ballot(next_pad);
+        gone_next = __ballot(next_pad != 0);
         // what the tile's scores have to be masked by
         bool masked = (gone & all) != 0 || static_cast<int>(j0) + KT - 1 > seen_all, values = false, none = MASK;
         uint32_t bits[KT / 32];
@@ -491,6 +493,8 @@ int launch_attn_forward_t(int dtype, const AttnParams& p, hipStream_t stream) {
 }
 
 #if TD_ATTN_TYPE == 0
+extern template int launch_attn_forward_t<f16>(int, const AttnParams&, hipStream_t);
+extern template int launch_attn_forward_t<bf16>(int, const AttnParams&, hipStream_t);
 template int launch_attn_forward_t<float>(int, const AttnParams&, hipStream_t);
 
 int64_t attn_forward_workspace(int dtype, const AttnParams& p) {

@@ -164,11 +164,6 @@ struct StagedRows {
                     if (!((gone >> row_of(u, t)) & 1)) r[u] = *reinterpret_cast<const u32x4*>(bytes + off[u]);
                 }
             }
-            if (D < DP) {
-#pragma unroll
-                for (int u = 0; u < kN; ++u)
-                    if (at_of(u, t) >= D * R::kS) r[u] = u32x4{0u, 0u, 0u, 0u};
-            }
         } else {
 #pragma unroll
             for (int u = 0; u < kN; ++u) {
@@ -179,7 +174,13 @@ struct StagedRows {
             }
         }
     }
-    __device__ __forceinline__ void store(unsigned char* tile, int t) const {
+    // The pieces past the row's end are cleared here and not in load(), where that would wait for the loads.
+    __device__ __forceinline__ void store(unsigned char* tile, int D, int t) {
+        if (VEC && D < DP) {
+#pragma unroll
+            for (int u = 0; u < kN; ++u)
+                if (at_of(u, t) >= D * R::kS) r[u] = u32x4{0u, 0u, 0u, 0u};
+        }
 #pragma unroll
         for (int u = 0; u < kN; ++u) *reinterpret_cast<u32x4*>(tile + row_of(u, t) * R::kPitch + at_of(u, t)) = r[u];
     }
