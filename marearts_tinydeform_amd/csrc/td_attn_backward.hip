@@ -126,17 +126,23 @@ __device__ __forceinline__ float ds_factor(const AttnParams& p, const RowInfo& i
     return __builtin_bit_cast(float, (254u - e) << 23);    // 2^(127 - e)
 }
 
-// dQ. The forward's shape: WK false, four wavefronts of 32 rows share the key tiles; WK true, 32 rows a workgroup and the
-// key tiles dealt to the wavefronts, whose sums are joined in LDS.
+// dQ. The forward's shape, WK: private key tiles, the wavefronts' sums joined in LDS.
 template <typename T, int DP, bool WK>
 constexpr int dq_key_tile() {
     return WK || DP * static_cast<int>(sizeof(T)) > 128 ? 32 : 64;
 }
-// Wavefronts a SIMD that the registers leave room for with few spills or none
-template <typename T, int DP, bool SLOW>
+// Wavefronts a SIMD that the registers leave room for with few spills or none. A workgroup of eight takes two of each SIMD.
+template <typename T, int DP, bool WK, bool SLOW>
 constexpr int dq_min_waves() {
     constexpr int bytes = DP * static_cast<int>(sizeof(T));
-    return bytes <= 64 ? (SLOW ? 2 : 3) : bytes <= 256 ? 2 : 1;
+    if (WK) return bytes <= 64 && !SLOW ? 3 : bytes <= 128 ? 2 : 1;
+    return bytes <= 64 || (bytes <= 128 && !SLOW) ? 4 : bytes <= 256 ? 2 : 1;
+}
+template <typename T, int DP, bool WK, bool SLOW>
+constexpr int dkv_min_waves() {
+    constexpr int bytes = DP * static_cast<int>(sizeof(T));
+    if (WK) return bytes <= 64 && !SLOW ? 3 : bytes <= 128 ? 2 : 1;
+    return bytes <= 64 && !SLOW ? 4 : bytes <= 256 ? 2 : 1;
 }
 
 // Sums over many keys (dQ) or rows (dK, dV) that are split over workgroups (TileSplit) leave float32 parts, which
@@ -194,11 +200,11 @@ void sum_parts(const AttnParams& p, const TileSplit& t, const float* part, void*
                        part, static_cast<T*>(out), quads, tile_rows, tiles, keys, p.D % 4 == 0);
 }
 template <typename T, int DP, bool WK, bool MASK, bool VEC>
-__global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dq_kernel(AttnParams p, RowInfo info,
+__global__ __launch_bounds__((kWaves<T, DP, WK> * kWave), (dq_min_waves<T, DP, WK, MASK>())) void attn_dq_kernel(AttnParams p, RowInfo info,
                                                                                     Parts parts, bool vec_out,
                                                                                     int tiles) {
     using R = TileRows<T, DP>;
-    constexpr int KT = dq_key_tile<T, DP, WK>(), NT = WK ? 64 : 256, ND = DP / 32;
+    constexpr int KT = dq_key_tile<T, DP, WK>(), ND = DP / 32, BM = kTileRows<T, DP, WK>;
     constexpr int kTile = KT * R::kPitch;
     extern __shared__ __align__(16) unsigned char lds[];
     const TileWork work = tile_work(parts.t);
@@ -207,11 +213,10 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dq_ke
     const int b = bh / p.Hk, hk = bh % p.Hk;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
     const int lane = threadIdx.x % kWave, half = lane >> 5;
-    const int t = WK ? lane : static_cast<int>(threadIdx.x);
     unsigned char* const kt_lds = lds + (WK ? wave * 2 * kTile : 0);
     unsigned char* const vt_lds = kt_lds + kTile;
 
-    const int row0 = tile * (WK ? 32 : 128), wrow0 = row0 + (WK ? 0 : wave * 32), r = wrow0 + (lane & 31);
+    const int row0 = tile * BM, wrow0 = row0 + (WK ? 0 : wave * 32), r = wrow0 + (lane & 31);
     const bool live = r < p.rows;
     const int i = static_cast<int>(fast_div(p.gdiv, static_cast<uint32_t>(live ? r : 0)));
     const int h = hk * p.G + (live ? r : 0) - i * p.G;
@@ -236,7 +241,7 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dq_ke
     const int diag = static_cast<int>(p.diag);
     const int last = p.causal ? i + diag : 2147483647;
     int kend = p.K;
-    const int top_row = (row0 + (WK ? 32 : 128) < p.rows ? row0 + (WK ? 32 : 128) : p.rows) - 1;
+    const int top_row = (row0 + BM < p.rows ? row0 + BM : p.rows) - 1;
     if (p.causal) {
         const int seen = static_cast<int>(fast_div(p.gdiv, static_cast<uint32_t>(top_row))) + diag + 1;
         kend = seen < kend ? seen : kend;
@@ -255,11 +260,10 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dq_ke
         if (lane < KT && j < kend) v = pad != nullptr ? pad[j] : 0;
         return v;
     };
-    StagedRows<T, DP, KT, NT, VEC> ks, vs;
+    TwoTiles<T, DP, KT, WK, VEC> staged;
     auto k_row = [&](int x) { return x * p.ks[1]; };
     auto v_row = [&](int x) { return x * p.vs[1]; };
-    ks.plan(k_row, p.D, t);
-    vs.plan(v_row, p.D, t);
+    staged.plan(k_row, v_row, p.D);
     f32x16 dq[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) dq[d] = f32x16{0.f};
@@ -278,15 +282,13 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dq_ke
         if constexpr (MASK)
 #pragma unroll
             for (int x = 0; x < KT / 32; ++x) mw[x] = mask_word(p, b, h, i, static_cast<int>(at / 32) + x);
-        ks.load(kb + at * p.ks[1], k_row, g & all, p.D, t);
-        vs.load(vb + at * p.vs[1], v_row, g & all, p.D, t);
+        staged.load(kb + at * p.ks[1], k_row, vb + at * p.vs[1], v_row, g & all, p.D);
     };
     if (j0 < kend) fetch(j0, gone);
     int next_pad = pad_byte(j0 + step);
     for (; j0 < kend; j0 += step) {
         if (!WK) __syncthreads();
-        ks.store(kt_lds, p.D, t);
-        vs.store(vt_lds, p.D, t);
+        staged.store(kt_lds, vt_lds, p.D);
         if (WK)
             wave_sync();
         else
@@ -378,8 +380,8 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dq_ke
     }
     if (!live) return;
     const float back = static_cast<float>(p.scale) / ds_scale * (kScaled<T> ? 0x1p-15f : 1.f);
-    const int64_t part_at = ((static_cast<int64_t>(work.tile - parts.t.whole) * work.parts + work.part) * (WK ? 32 : 128) +
-                             r - row0) * p.D;
+    const int64_t part_at = ((static_cast<int64_t>(work.tile - parts.t.whole) * work.parts + work.part) * BM + r -
+                             row0) * p.D;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -392,8 +394,7 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dq_ke
         }
 }
 
-// dK and dV. WK false: four wavefronts of 32 keys each share the row tiles. WK true: 32 keys a workgroup and the row tiles
-// dealt to the wavefronts. The scores stand untransposed here (a lane's column is its key), so that P and dS are operands
+// dK and dV. WK: private row tiles. The scores stand untransposed here (a lane's column is its key), so that P and dS are operands
 // of dV^T = g^T P and dK^T = Q^T dS as they stand. Rows past the end hold zeros and m = inf: P = 0.
 template <typename T, int DP, bool WK>
 constexpr int dkv_row_tile() {
@@ -406,20 +407,21 @@ template <typename T, int DP, bool WK>
 constexpr bool v_in_lds() {
     return !WK && DP * static_cast<int>(sizeof(T)) == 256;
 }
-template <bool WK, bool MASK>
+template <typename T, int DP, bool WK, bool MASK>
 constexpr int dkv_row_bytes() {
-    return 12 + (WK ? 4 : 16) + (MASK ? 8 + (WK ? 4 : 16) : 0) + (WK ? 0 : 4);  // a multiple of 8
+    constexpr int words = kTileRows<T, DP, WK> / 8;  // bytes
+    return 12 + words + (MASK ? 8 + words : 0) + (words == 4 ? 0 : 4);  // a multiple of 4 that leaves tiles 16-byte aligned
 }
 
 template <typename T, int DP, bool WK, bool MASK, bool VEC>
-__global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dkv_kernel(AttnParams p, RowInfo info,
+__global__ __launch_bounds__((kWaves<T, DP, WK> * kWave), (dkv_min_waves<T, DP, WK, MASK>())) void attn_dkv_kernel(AttnParams p, RowInfo info,
                                                                                      Parts parts, bool vec_out,
                                                                                      int tiles) {
     using R = TileRows<T, DP>;
-    constexpr int RT = dkv_row_tile<T, DP, WK>(), NT = WK ? 64 : 256, ND = DP / 32;
+    constexpr int RT = dkv_row_tile<T, DP, WK>(), ND = DP / 32, BM = kTileRows<T, DP, WK>;
     constexpr int kTile = RT * R::kPitch;
-    constexpr int KW = WK ? 1 : 4;  // words of 32 keys that the workgroup's keys have
-    constexpr int kArea = 2 * kTile + RT * dkv_row_bytes<WK, MASK>();
+    constexpr int KW = BM / 32;  // words of 32 keys that the workgroup's keys have
+    constexpr int kArea = 2 * kTile + RT * dkv_row_bytes<T, DP, WK, MASK>();
     extern __shared__ __align__(16) unsigned char lds[];
     const TileWork work = tile_work(parts.t);
     if (work.tile < 0) return;
@@ -438,7 +440,7 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dkv_k
     int64_t* const o_lds = reinterpret_cast<int64_t*>(k_lds + KW * RT);
 
     // the lane's key
-    const int key0 = tile * (WK ? 32 : 128), wkey0 = key0 + (WK ? 0 : wave * 32), j = wkey0 + (lane & 31);
+    const int key0 = tile * BM, wkey0 = key0 + (WK ? 0 : wave * 32), j = wkey0 + (lane & 31);
     const bool live = j < p.K && (p.pad == nullptr || p.pad[static_cast<int64_t>(b) * p.K + j] == 0);
     constexpr bool kVInLds = v_in_lds<T, DP, WK>();
     u32x4 kf[R::kChunks], vf[kVInLds ? 1 : R::kChunks];
@@ -474,7 +476,7 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dkv_k
     const int64_t gs1 = static_cast<int64_t>(p.H) * p.D, gs2 = p.D;
     const T* const gb = static_cast<const T*>(p.go) + b * p.Q * gs1 + hk * p.G * gs2;
     const f32x4* const ib = info.rows + static_cast<int64_t>(bh) * p.rows;
-    StagedRows<T, DP, RT, NT, VEC> qs, gs;
+    TwoTiles<T, DP, RT, WK, VEC> staged;
     // rows of a tile lie the same in every tile when the heads of a key head divide it
     const bool even = RT % p.G == 0;
     int64_t from_row = 0;
@@ -494,10 +496,7 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dkv_k
         split_row(x, i, g);
         return i * gs1 + g * gs2;
     };
-    if (even) {
-        qs.plan(q_row, p.D, t);
-        gs.plan(g_row, p.D, t);
-    }
+    if (even) staged.plan(q_row, g_row, p.D);
     f32x4 ri = f32x4{0.f, 0.f, 0.f, 0.f};
     int64_t mo = 0;
     MaskWord words[KW] = {};
@@ -508,13 +507,9 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dkv_k
         from_row = at;
         const int64_t left = p.rows - at;
         const uint64_t gone = left >= RT ? 0 : ~uint64_t{0} << left;
-        if (!even) {
-            qs.plan(q_row, p.D, t);
-            gs.plan(g_row, p.D, t);
-        }
+        if (!even) staged.plan(q_row, g_row, p.D);
         const int64_t i0 = fast_div(p.gdiv, static_cast<uint32_t>(at));
-        qs.load(qb + i0 * p.qs[1], q_row, gone, p.D, t);
-        gs.load(gb + i0 * gs1, g_row, gone, p.D, t);
+        staged.load(qb + i0 * p.qs[1], q_row, gb + i0 * gs1, g_row, gone, p.D);
         if (t < RT) {
             const bool in = in_rows = t < left;
             ri = in ? ib[at + t] : f32x4{__builtin_inff(), 0.f, 0.f, 0.f};
@@ -544,8 +539,7 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dkv_k
     if (r0 < rend) fetch(r0);
     for (; r0 < rend; r0 += step) {
         if (!WK) __syncthreads();
-        qs.store(q_lds, p.D, t);
-        gs.store(g_lds, p.D, t);
+        staged.store(q_lds, g_lds, p.D);
         if (t < RT) {
             m_lds[t] = apart ? ri[0] : ri[0] + ri[1] - kPShift<T>;
             l_lds[t] = ri[1] - kPShift<T>;
@@ -671,8 +665,8 @@ __global__ __launch_bounds__(256, (dq_min_waves<T, DP, MASK>())) void attn_dkv_k
     const float pv = live ? (kScaled<T> ? 0x1p-15f : 1.f) : 0.f;
     const float back = static_cast<float>(p.scale) / ds_scale * (kScaled<T> ? 0x1p-15f : 1.f);
     const int64_t at = ((static_cast<int64_t>(b) * p.K + j) * p.Hk + hk) * p.D;
-    const int64_t part_at = ((static_cast<int64_t>(work.tile - parts.t.whole) * work.parts + work.part) * (WK ? 32 : 128) +
-                             j - key0) * p.D;
+    const int64_t part_at = ((static_cast<int64_t>(work.tile - parts.t.whole) * work.parts + work.part) * BM + j -
+                             key0) * p.D;
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
         if (!live) dk[d] = dv[d] = f32x16{0.f};  // a key that nobody sees: its column may hold anything
@@ -694,10 +688,9 @@ struct BackShape {
     bool vec;
     struct One {
         bool wk;
-        int tiles;
+        int tile_rows, tiles;
         TileSplit t;
-        int tile_rows() const { return wk ? 32 : 128; }
-        int64_t part_floats(int D) const { return static_cast<int64_t>(t.total - t.whole) * t.n * tile_rows() * D; }
+        int64_t part_floats(int D) const { return static_cast<int64_t>(t.total - t.whole) * t.n * tile_rows * D; }
     } q, k;
 };
 
@@ -713,7 +706,7 @@ bool back_vec(int dtype, const AttnParams& p) {
            static_cast<int64_t>(p.H) * p.D < (int64_t{1} << 31) / (128 * elem);
 }
 
-// Workgroups of 128 rows (keys) that share tiles, when they fill the GPU twice; else of 32 rows (keys) with the others'
+// Workgroups of 256 rows (keys) that share tiles, when they fill the GPU; else of 32 rows (keys) with the others'
 // tiles over the wavefronts, which needs no second launch, for heads whose private tiles fit in the registers. Where that
 // still leaves CUs without work and the loops are long, parts; where many tiles leave a few over, parts of those
 // (even_split).
@@ -725,11 +718,13 @@ BackShape back_shape(int dtype, const AttnParams& p, bool vec) {
     auto shape = [&](int n, int over) {
         BackShape::One o{};
         o.wk = can && heads * ((n + 127) / 128) < 512;
-        o.tiles = o.wk ? (n + 31) / 32 : (n + 127) / 128;
+        o.tile_rows = tile_rows(o.wk, padded_width(p.D) * elem_size(dtype));
+        o.tiles = (n + o.tile_rows - 1) / o.tile_rows;
         const int total = static_cast<int>(heads * o.tiles);
         o.t = TileSplit{1, total, total};
-        if (total > 0 && total < 384) {
-            const int want = (1024 + total - 1) / total, most = over / 512;  // 4 steps of 4 x 32 or 16 of 32 a part
+        const int few = o.tile_rows == 256 ? 256 : 384;
+        if (total > 0 && total < few) {
+            const int want = ((o.tile_rows == 256 ? 512 : 1024) + total - 1) / total, most = over / 512;  // 4 steps of 4 x 32 or 16 of 32 a part
             const int parts = want < most ? want : most;
             if (parts > 1) o.t = TileSplit{parts, 0, total};
         } else if (!o.wk && !p.causal) {
@@ -755,17 +750,18 @@ int run_dq(const AttnParams& p, const BackShape& s, const RowInfo& info, float* 
     if (e != hipSuccess) return set_error(TD_E_LAUNCH, "attention backward: LDS size: %s", hipGetErrorString(e));
     const bool vec_out = p.D % 4 == 0 && reinterpret_cast<uintptr_t>(p.dq) % (4 * sizeof(T)) == 0;
     const Parts parts{s.q.t, ws, nullptr};
-    hipLaunchKernelGGL(fn, dim3(tile_grid(s.q.t)), dim3(256), bytes, stream, p, info, parts, vec_out, s.q.tiles);
-    if (s.q.t.n > 1) sum_parts<T>(p, s.q.t, parts.a, p.dq, s.q.tile_rows(), s.q.tiles, false, stream);
+    hipLaunchKernelGGL(fn, dim3(tile_grid(s.q.t)), dim3(kWaves<T, DP, WK> * kWave), bytes, stream, p, info, parts, vec_out,
+                       s.q.tiles);
+    if (s.q.t.n > 1) sum_parts<T>(p, s.q.t, parts.a, p.dq, s.q.tile_rows, s.q.tiles, false, stream);
     return 0;
 }
 
 template <typename T, int DP, bool WK, bool MASK, bool VEC>
 int run_dkv(const AttnParams& p, const BackShape& s, const RowInfo& info, float* ws, hipStream_t stream) {
     static std::atomic<uint64_t> done{0};
-    constexpr int RT = dkv_row_tile<T, DP, WK>(), area = 2 * RT * TileRows<T, DP>::kPitch + RT * dkv_row_bytes<WK, MASK>();
+    constexpr int RT = dkv_row_tile<T, DP, WK>(), area = 2 * RT * TileRows<T, DP>::kPitch + RT * dkv_row_bytes<T, DP, WK, MASK>();
     constexpr int join = 2 * 32 * (DP + 4) * 4;
-    constexpr int own = v_in_lds<T, DP, WK>() ? 128 * TileRows<T, DP>::kPitch : 0;
+    constexpr int own = v_in_lds<T, DP, WK>() ? kTileRows<T, DP, WK> * TileRows<T, DP>::kPitch : 0;
     constexpr int bytes = WK ? (4 * area > join ? 4 * area : join) : area + own;
     static_assert(bytes <= 160 * 1024, "LDS of a CU");
     auto* const fn = &attn_dkv_kernel<T, DP, WK, MASK, VEC>;
@@ -775,10 +771,11 @@ int run_dkv(const AttnParams& p, const BackShape& s, const RowInfo& info, float*
     const bool vec_out = p.D % 4 == 0 && reinterpret_cast<uintptr_t>(p.dk) % (4 * sizeof(T)) == 0 &&
                          reinterpret_cast<uintptr_t>(p.dv) % (4 * sizeof(T)) == 0;
     const Parts parts{s.k.t, ws, ws + s.k.part_floats(p.D)};
-    hipLaunchKernelGGL(fn, dim3(tile_grid(s.k.t)), dim3(256), bytes, stream, p, info, parts, vec_out, s.k.tiles);
+    hipLaunchKernelGGL(fn, dim3(tile_grid(s.k.t)), dim3(kWaves<T, DP, WK> * kWave), bytes, stream, p, info, parts, vec_out,
+                       s.k.tiles);
     if (s.k.t.n > 1) {
-        sum_parts<T>(p, s.k.t, parts.a, p.dk, s.k.tile_rows(), s.k.tiles, true, stream);
-        sum_parts<T>(p, s.k.t, parts.b, p.dv, s.k.tile_rows(), s.k.tiles, true, stream);
+        sum_parts<T>(p, s.k.t, parts.a, p.dk, s.k.tile_rows, s.k.tiles, true, stream);
+        sum_parts<T>(p, s.k.t, parts.b, p.dv, s.k.tile_rows, s.k.tiles, true, stream);
     }
     return 0;
 }

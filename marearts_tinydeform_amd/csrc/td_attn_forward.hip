@@ -35,31 +35,21 @@ constexpr int key_tile() {
     return WK || DP * static_cast<int>(sizeof(T)) > 256 ? 32 : 64;
 }
 
-// Wavefronts a SIMD that the registers have to leave room for (without spills)
+// Wavefronts a SIMD that the registers have to leave room for. A workgroup of eight takes two of each SIMD.
 template <typename T, int DP, bool WK, bool SLOW>
 constexpr int min_waves() {
     constexpr int bytes = DP * static_cast<int>(sizeof(T));
-    constexpr int n = bytes <= 64 ? 4 : bytes <= 128 ? 3 : bytes <= 256 ? 2 : 1;
-    return n > 1 && bytes <= 128 && (WK || SLOW) ? n - 1 : SLOW ? 1 : n;
+    if (WK) return bytes <= 64 ? 3 : bytes <= 128 ? 2 : SLOW ? 1 : 2;
+    return bytes <= 64 || (bytes <= 128 && !SLOW) ? 4 : bytes <= 256 ? 2 : 1;
 }
 
-// 16-bit rows of up to 64 elements: the kernel is bound by the vector units (a score takes a fused multiply-add, an
-// exponential at a quarter of the rate, half a maximum, half a conversion and an addition: 28 cycles of a SIMD, its share
-// of the products 8 or 16), and l is summed by the matrix units, as one more column of ones of V. It is then the sum of
-// the rounded probabilities, which is also what O is a sum of.
-template <typename T, int DP, bool WK>
-constexpr bool sum_by_mma() {
-    return sizeof(T) == 2 && DP <= 64 && !WK;
-}
-
-// WK false: four wavefronts of 32 rows each share the key tiles of the workgroup's 128 rows. WK true: the workgroup has
-// 32 rows and each wavefront every fourth key tile, in LDS of its own; the four partial results are joined in LDS.
+// WK: private key tiles (TwoTiles); the four wavefronts' partial results are joined in LDS.
 // MASK: there is a mask tensor. VEC: operands are read 16 bytes at a time (StagedRows).
 template <typename T, int DP, bool WK, bool MASK, bool VEC>
-__global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forward_kernel(AttnParams p, Split sp, bool vec_out,
+__global__ __launch_bounds__((kWaves<T, DP, WK> * kWave), (min_waves<T, DP, WK, MASK>())) void attn_forward_kernel(AttnParams p, Split sp, bool vec_out,
                                                                                int tiles) {
     using R = TileRows<T, DP>;
-    constexpr int KT = key_tile<T, DP, WK>(), NT = WK ? 64 : 256, ND = DP / 32;
+    constexpr int KT = key_tile<T, DP, WK>(), ND = DP / 32, BM = kTileRows<T, DP, WK>;
     constexpr int kTile = KT * R::kPitch;
     extern __shared__ __align__(16) unsigned char lds[];
     const TileWork work = tile_work(sp.t);
@@ -68,12 +58,11 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
     const int b = bh / p.Hk, hk = bh % p.Hk;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
     const int lane = threadIdx.x % kWave, half = lane >> 5;
-    const int t = WK ? lane : static_cast<int>(threadIdx.x);
     unsigned char* const kt_lds = lds + (WK ? wave * 2 * kTile : 0);
     unsigned char* const vt_lds = kt_lds + kTile;
 
     // the lane's row
-    const int row0 = tile * (WK ? 32 : 128), wrow0 = row0 + (WK ? 0 : wave * 32), r = wrow0 + (lane & 31);
+    const int row0 = tile * BM, wrow0 = row0 + (WK ? 0 : wave * 32), r = wrow0 + (lane & 31);
     const bool live = r < p.rows;
     const int i = static_cast<int>(fast_div(p.gdiv, static_cast<uint32_t>(live ? r : 0)));
     const int h = hk * p.G + (live ? r : 0) - i * p.G;
@@ -90,7 +79,7 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
 
     // the workgroup's keys, and the wavefront's first and last row's
     int kend = p.K, k0 = 0;
-    const int top_row = (row0 + (WK ? 32 : 128) < p.rows ? row0 + (WK ? 32 : 128) : p.rows) - 1;
+    const int top_row = (row0 + BM < p.rows ? row0 + BM : p.rows) - 1;
     if (p.causal) {
         const int seen = static_cast<int>(fast_div(p.gdiv, static_cast<uint32_t>(top_row))) + diag + 1;
         kend = seen < kend ? seen : kend;
@@ -115,21 +104,14 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
         return v;
     };
 
-    StagedRows<T, DP, KT, NT, VEC> ks, vs;
+    TwoTiles<T, DP, KT, WK, VEC> staged;
     auto k_row = [&](int x) { return x * p.ks[1]; };
     auto v_row = [&](int x) { return x * p.vs[1]; };
-    ks.plan(k_row, p.D, t);
-    vs.plan(v_row, p.D, t);
+    staged.plan(k_row, v_row, p.D);
     float m = kNegInf, l = 0.f;
-    f32x16 o[ND], lm = f32x16{0.f};
+    f32x16 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = f32x16{0.f};
-    constexpr bool kSumMma = sum_by_mma<T, DP, WK>();
-    u32x4 ones = {0u, 0u, 0u, 0u};
-    if constexpr (kSumMma) {
-        const unsigned short one = __builtin_bit_cast(unsigned short, static_cast<T>(1.f));
-        ones = u32x4{1u, 1u, 1u, 1u} * (one * 0x10001u);
-    }
 
     constexpr int step = WK ? 4 * KT : KT;
     constexpr uint64_t all = KT == 64 ? ~uint64_t{0} : (uint64_t{1} << (KT & 63)) - 1;
@@ -140,15 +122,13 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
         if constexpr (MASK)
 #pragma unroll
             for (int x = 0; x < KT / 32; ++x) mw[x] = mask_word(p, b, h, i, static_cast<int>(at / 32) + x);
-        ks.load(kb + at * p.ks[1], k_row, g & all, p.D, t);
-        vs.load(vb + at * p.vs[1], v_row, g & all, p.D, t);
+        staged.load(kb + at * p.ks[1], k_row, vb + at * p.vs[1], v_row, g & all, p.D);
     };
     if (j0 < kend) fetch(j0, gone);
     int next_pad = pad_byte(j0 + step);
     for (; j0 < kend; j0 += step) {
         if (!WK) __syncthreads();
-        ks.store(kt_lds, p.D, t);
-        vs.store(vt_lds, p.D, t);
+        staged.store(kt_lds, vt_lds, p.D);
         if (WK)
             wave_sync();
         else
@@ -199,10 +179,7 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
                 const float to = __builtin_fmaxf(m, mt);
                 const float shrink = to == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m - to);
                 m = to;
-                if constexpr (kSumMma)
-                    lm *= shrink;
-                else
-                    l *= shrink;
+                l *= shrink;
 #pragma unroll
                 for (int d = 0; d < ND; ++d) o[d] *= shrink;
             }
@@ -213,13 +190,10 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     pr[e] = __builtin_amdgcn_exp2f(fmaf(s[x][e], cc, -from));
-                    if constexpr (!kSumMma) l += pr[e];
+                    l += pr[e];
                 }
                 typename R::Packed w[R::kPacked];
                 R::pack(pr, w);
-                if constexpr (kSumMma)
-#pragma unroll
-                    for (int y = 0; y < R::kPacked; ++y) lm = Mma<T>::mul(ones, w[y], lm);
 #pragma unroll
                 for (int d = 0; d < ND; ++d) o[d] = R::columns(vt_lds, 32 * x, 32 * d, lane, w, o[d]);
             }
@@ -227,7 +201,7 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
         gone = gone_next;
         if (WK) wave_sync();
     }
-    l = kSumMma ? lm[0] : l + other_half(l);
+    l += other_half(l);
 
     if constexpr (WK) {
         // join the four wavefronts' parts: maxima and sums first, then each scaled O, through LDS
@@ -284,8 +258,7 @@ __global__ __launch_bounds__(256, (min_waves<T, DP, WK, MASK>())) void attn_forw
 
     const int64_t row = (static_cast<int64_t>(b) * p.H + h) * p.Q + i;
     if (work.parts > 1) {
-        const int64_t part = (static_cast<int64_t>(work.tile - sp.t.whole) * work.parts + work.part) * (WK ? 32 : 128) +
-                             (r - row0);
+        const int64_t part = (static_cast<int64_t>(work.tile - sp.t.whole) * work.parts + work.part) * BM + r - row0;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -393,14 +366,13 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p, Split sp, 
     }
 }
 
-// The launch shape. Workgroups of 128 rows that share key tiles, when they fill the GPU twice, with what is left over after
-// an even share for every CU split (even_split); else workgroups of 32 rows with the keys over the wavefronts, and when
+// The launch shape. Workgroups of 256 rows that share key tiles, when they fill the GPU, with what is left over after an
+// even share for every CU split (even_split); else workgroups of 32 rows with the keys over the wavefronts, and when
 // those are few and the keys many, the keys over several workgroups too.
 struct Shape {
     bool vec, wk;
-    int tiles, keys;
+    int tile_rows, tiles, keys;
     TileSplit t;
-    int tile_rows() const { return wk ? 32 : 128; }
 };
 
 Shape shape_of(int dtype, const AttnParams& p) {
@@ -414,11 +386,13 @@ Shape shape_of(int dtype, const AttnParams& p) {
     const int64_t heads = static_cast<int64_t>(p.B) * p.Hk;
     const bool can = s.vec && padded_width(p.D) * elem <= 256;  // wider rows' private tiles do not fit in registers
     s.wk = can && heads * ((p.rows + 127) / 128) < 512;
-    s.tiles = s.wk ? (p.rows + 31) / 32 : (p.rows + 127) / 128;
+    s.tile_rows = tile_rows(s.wk, padded_width(p.D) * elem);
+    s.tiles = (p.rows + s.tile_rows - 1) / s.tile_rows;
     const int total = static_cast<int>(heads * s.tiles);
     s.t = TileSplit{1, total, total};
-    if (total < 512 && p.K > 1024) {
-        int64_t n = (1024 + total - 1) / total;
+    const int few = s.tile_rows == 256 ? 256 : 512;  // workgroups that a CU's worth of work takes
+    if (total < few && p.K > 1024) {
+        int64_t n = (2 * few + total - 1) / total;
         const int64_t most = (p.K + 511) / 512;
         n = n < most ? n : most;
         n = n < kJoinParts ? n : kJoinParts;
@@ -433,7 +407,7 @@ Shape shape_of(int dtype, const AttnParams& p) {
 
 // Floats that the parts take: their outputs, maxima and sums
 int64_t part_floats(const AttnParams& p, const Shape& s) {
-    return static_cast<int64_t>(s.t.total - s.t.whole) * s.t.n * s.tile_rows() * (p.D + 2);
+    return static_cast<int64_t>(s.t.total - s.t.whole) * s.t.n * s.tile_rows * (p.D + 2);
 }
 
 template <typename T, int DP, bool WK, bool MASK, bool VEC>
@@ -449,12 +423,12 @@ int run(const AttnParams& p, const Shape& s, const Split& sp, hipStream_t stream
     if (e != hipSuccess) return set_error(TD_E_LAUNCH, "attention: LDS size: %s", hipGetErrorString(e));
     const bool vec_out = p.D % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.out_low)) %
                                                  (4 * sizeof(T)) == 0;
-    hipLaunchKernelGGL(fn, dim3(tile_grid(sp.t)), dim3(256), bytes, stream, p, sp, vec_out, s.tiles);
+    hipLaunchKernelGGL(fn, dim3(tile_grid(sp.t)), dim3(kWaves<T, DP, WK> * kWave), bytes, stream, p, sp, vec_out, s.tiles);
     if (sp.t.n > 1) {
         const int rows = sp.t.n <= 16 ? 256 / padded_width(p.D) : 1;  // of a workgroup; a tile's are a multiple of it
-        const int64_t groups = static_cast<int64_t>(sp.t.total - sp.t.whole) * s.tile_rows() / rows;
+        const int64_t groups = static_cast<int64_t>(sp.t.total - sp.t.whole) * s.tile_rows / rows;
         hipLaunchKernelGGL((attn_join_kernel<T>), dim3(static_cast<unsigned>(groups)), dim3(256), 0, stream, p, sp,
-                           padded_width(p.D), rows, s.tile_rows(), s.tiles);
+                           padded_width(p.D), rows, s.tile_rows, s.tiles);
     }
     const hipError_t le = hipGetLastError();
     return le == hipSuccess ? 0 : set_error(TD_E_LAUNCH, "attention launch failed: %s", hipGetErrorString(le));

@@ -186,6 +186,57 @@ struct StagedRows {
     }
 };
 
+// Workgroups. Shared: eight wavefronts of 32 rows (or keys) each share the tiles of the other side, the first four staging
+// one of the two operands and the others the second. Staging and its barriers take a fifth of the time of four such
+// wavefronts (they were left out to see: 8192 tokens x 8 heads of 32 273 -> 232 us, 4096 x 16 of 128 334 -> 272), and
+// eight do it half as often for a row; rows of more than 256 bytes leave registers for four only. Private: four
+// wavefronts have the same 32 rows (or keys) and every fourth tile each, staged by itself alone, for problems of few rows
+// (keys).
+constexpr int shared_waves(int row_bytes) { return row_bytes > 256 ? 4 : 8; }
+template <typename T, int DP, bool PRIVATE>
+constexpr int kWaves = PRIVATE ? 4 : shared_waves(DP * static_cast<int>(sizeof(T)));
+template <typename T, int DP, bool PRIVATE>
+constexpr int kTileRows = PRIVATE ? 32 : 32 * kWaves<T, DP, PRIVATE>;
+inline int tile_rows(bool is_private, int row_bytes) { return is_private ? 32 : 32 * shared_waves(row_bytes); }
+
+template <typename T, int DP, int NR, bool PRIVATE, bool VEC>
+struct TwoTiles {
+    static constexpr bool kBoth = kWaves<T, DP, PRIVATE> == 4;  // a thread stages both operands
+    static constexpr int kThreads = PRIVATE ? 64 : 256;
+    StagedRows<T, DP, NR, kThreads, VEC> a, b;  // not both: a alone, of the operand that the wavefront stages
+    int t;
+    bool second;
+    __device__ __forceinline__ TwoTiles() : t(static_cast<int>(threadIdx.x) & (kThreads - 1)) {
+        second = __builtin_amdgcn_readfirstlane(!kBoth && threadIdx.x >= 256);
+    }
+    template <typename F, typename G>
+    __device__ __forceinline__ void plan(F f, G g, int D) {
+        if constexpr (kBoth) {
+            a.plan(f, D, t);
+            b.plan(g, D, t);
+        } else {
+            a.plan([&](int x) { return second ? g(x) : f(x); }, D, t);
+        }
+    }
+    template <typename F, typename G>
+    __device__ __forceinline__ void load(const T* base_a, F f, const T* base_b, G g, uint64_t gone, int D) {
+        if constexpr (kBoth) {
+            a.load(base_a, f, gone, D, t);
+            b.load(base_b, g, gone, D, t);
+        } else {
+            a.load(second ? base_b : base_a, [&](int x) { return second ? g(x) : f(x); }, gone, D, t);
+        }
+    }
+    __device__ __forceinline__ void store(unsigned char* tile_a, unsigned char* tile_b, int D) {
+        if constexpr (kBoth) {
+            a.store(tile_a, D, t);
+            b.store(tile_b, D, t);
+        } else {
+            a.store(second ? tile_b : tile_a, D, t);
+        }
+    }
+};
+
 // Orders a wavefront's LDS accesses before it against those after it. The LDS serves one wavefront's accesses in order,
 // so this keeps the compiler from moving them and costs nothing.
 __device__ __forceinline__ void wave_sync() {
@@ -225,12 +276,12 @@ inline unsigned tile_grid(const TileSplit& s) {
     return xcd_grid(s.whole) + (s.n > 1 ? xcd_grid(static_cast<int64_t>(s.total - s.whole) * s.n) : 0);
 }
 // Every CU works at its own rate whether it holds four workgroups or one, so 4 1/8 tiles a CU take as long as 5. Where a
-// few tiles are left over after an even share for every CU, those are split over all CUs (8400 tokens of 16 heads are
-// 1056 tiles on 256 CUs: 322 us with the 32 left over whole, ... split).
+// few tiles are left over after an even share for every CU, those are split over all CUs (8400 tokens of 16 heads as 1056
+// tiles of 128 rows on 256 CUs: 322 us with the 32 left over whole, 288 split).
 inline TileSplit even_split(int total, int steps) {
     const int cus = cu_count(), rest = total % cus;
     TileSplit s{1, total, total};
-    if (total < 2 * cus || total > 8 * cus || rest == 0 || rest > cus / 2) return s;
+    if (total < cus || total > 8 * cus || rest == 0 || rest > cus / 2) return s;
     int n = cus / rest;
     n = n < 8 ? n : 8;
     n = n < steps / 4 ? n : steps / 4;
