@@ -2,7 +2,11 @@
 
 Drop-in for marearts_tinydeform (same functions, arguments, results and errors; reference
 marearts_tinydeform/__init__.py:12-79). GPU tensors run hand-written HIP kernels for gfx950 through the C ABI of
-libtinydeform.so; CPU tensors run the PyTorch reference path. Inference only.
+libtinydeform.so; CPU tensors run the PyTorch reference path.
+
+Beside the operator stands what the rest of such a decoder layer runs: ma_attn, attention among the queries or any other
+tokens, and ma_layer_norm, the norm after a sublayer, each with a training form (ma_attn_train, ma_layer_norm_train), and
+DeformDecoderLayer, the whole layer on them.
 """
 
 import functools
@@ -19,7 +23,8 @@ from .reference import (layer_locations_reference, ma_attn_reference, ma_deform_
 __all__ = ['ma_deform_attn', 'ma_deform_attn_reference', 'choose_mode', 'ma_deform_sample', 'ma_deform_sample_v2',
            'predict_us', 'cost_features', 'gap_features', 'ma_deform_attn_layer', 'ma_deform_attn_layer_reference', 'layer_locations_reference',
            'MSDeformAttnLayer', 'ma_deform_attn_train', 'ma_deform_sample_train', 'ma_attn', 'ma_attn_train',
-           'ma_attn_reference', 'ma_layer_norm', 'ma_layer_norm_train', 'ma_layer_norm_reference']
+           'ma_attn_reference', 'ma_layer_norm', 'ma_layer_norm_train', 'ma_layer_norm_reference', 'SelfAttnLayer',
+           'DeformDecoderLayer']
 __version__ = '0.1.1'  # the version of the reference API this package implements (marearts_tinydeform 0.1.1)
 
 MODES = ('auto', 'fused', 'project')
@@ -522,3 +527,94 @@ class MSDeformAttnLayer(torch.nn.Module):
             self.attention_weights.bias, self.value_proj.weight, self.value_proj.bias, self.output_proj.weight,
             self.output_proj.bias, self.n_heads, self.n_points, position_embeddings=position_embeddings,
             padding_mask=padding_mask, mode=self.mode, return_attention_weights=True)
+
+
+def _trains(module, *tensors):
+    return torch.is_grad_enabled() and (any(t.requires_grad for t in module.parameters()) or any(
+        t is not None and t.requires_grad for t in tensors))
+
+
+class SelfAttnLayer(torch.nn.Module):
+    """Self-attention among a DETR decoder's queries, running ma_attn (ma_attn_train where gradients are asked for).
+
+    Same submodules as HF transformers' RTDetrSelfAttention (k_proj, v_proj, q_proj, o_proj), so its state dict loads
+    unchanged. The position embeddings are added to what the queries and keys are projected from, not to the values.
+    attention_mask and key_padding_mask are ma_attn's attn_mask and key_padding_mask (True: may not attend). Returns
+    (output [B, Q, d_model], None): the probabilities are never stored.
+    """
+
+    def __init__(self, d_model=256, n_heads=8):
+        super().__init__()
+        if d_model % n_heads != 0:
+            raise ValueError(f'd_model ({d_model}) must be divisible by n_heads ({n_heads})')
+        self.d_model, self.n_heads = d_model, n_heads
+        self.k_proj = torch.nn.Linear(d_model, d_model)
+        self.v_proj = torch.nn.Linear(d_model, d_model)
+        self.q_proj = torch.nn.Linear(d_model, d_model)
+        self.o_proj = torch.nn.Linear(d_model, d_model)
+        self.reset_parameters()
+
+    @torch.no_grad()
+    def reset_parameters(self):
+        for lin in (self.k_proj, self.v_proj, self.q_proj, self.o_proj):
+            torch.nn.init.xavier_uniform_(lin.weight)
+            torch.nn.init.zeros_(lin.bias)
+
+    def forward(self, hidden_states, attention_mask=None, position_embeddings=None, key_padding_mask=None, **kwargs):
+        attend = ma_attn_train if _trains(self, hidden_states, position_embeddings) else ma_attn
+        placed = hidden_states if position_embeddings is None else hidden_states + position_embeddings
+        heads = hidden_states.shape[:2] + (self.n_heads, self.d_model // self.n_heads)
+        out = attend(self.q_proj(placed).view(heads), self.k_proj(placed).view(heads),
+                     self.v_proj(hidden_states).view(heads), attn_mask=attention_mask,
+                     key_padding_mask=key_padding_mask)
+        return self.o_proj(out), None
+
+
+class _Mlp(torch.nn.Module):
+    def __init__(self, d_model, ffn_dim):
+        super().__init__()
+        self.fc1 = torch.nn.Linear(d_model, ffn_dim)
+        self.fc2 = torch.nn.Linear(ffn_dim, d_model)
+
+    def forward(self, x):
+        return self.fc2(torch.relu_(self.fc1(x)))
+
+
+class DeformDecoderLayer(torch.nn.Module):
+    """A whole DETR decoder layer: self-attention among the queries (ma_attn), deformable cross-attention
+    (MSDeformAttnLayer) and the feed-forward layers, each followed by a layer norm of the sum with its input
+    (ma_layer_norm). Where gradients are asked for, the same on ma_attn_train and ma_layer_norm_train.
+
+    Same submodules as HF transformers' RTDetrDecoderLayer, so its state dict loads unchanged (ReLU, no dropout), and the
+    same forward arguments and result. encoder_attention_mask is, as there, the mask among the queries (denoising groups):
+    ma_attn's attn_mask, added where it is of the inputs' dtype, True for "may not attend" where it is bool. Beside those,
+    query_padding_mask [B, Q] marks padded queries (no query attends to them) and memory_padding_mask [B, N] padded
+    tokens of the encoder's output, both True for padding.
+    """
+
+    def __init__(self, d_model=256, n_levels=4, n_heads=8, n_points=4, ffn_dim=1024, eps=1e-5, mode='auto'):
+        super().__init__()
+        self.self_attn = SelfAttnLayer(d_model, n_heads)
+        self.self_attn_layer_norm = torch.nn.LayerNorm(d_model, eps=eps)
+        self.encoder_attn = MSDeformAttnLayer(d_model, n_levels, n_heads, n_points, mode)
+        self.encoder_attn_layer_norm = torch.nn.LayerNorm(d_model, eps=eps)
+        self.mlp = _Mlp(d_model, ffn_dim)
+        self.final_layer_norm = torch.nn.LayerNorm(d_model, eps=eps)
+
+    def forward(self, hidden_states, object_queries_position_embeddings=None, reference_points=None,
+                spatial_shapes=None, spatial_shapes_list=None, level_start_index=None, encoder_hidden_states=None,
+                encoder_attention_mask=None, query_padding_mask=None, memory_padding_mask=None, **kwargs):
+        pos = object_queries_position_embeddings
+        norm = ma_layer_norm_train if _trains(self, hidden_states, pos, reference_points,
+                                              encoder_hidden_states) else ma_layer_norm
+
+        def after(ln, x, sublayer):
+            return norm(sublayer, ln.weight, ln.bias, residual=x, eps=ln.eps)
+
+        x = hidden_states
+        x = after(self.self_attn_layer_norm, x, self.self_attn(x, encoder_attention_mask, pos, query_padding_mask)[0])
+        x = after(self.encoder_attn_layer_norm, x, self.encoder_attn(
+            x, attention_mask=None if memory_padding_mask is None else ~memory_padding_mask.bool(),
+            encoder_hidden_states=encoder_hidden_states, position_embeddings=pos, reference_points=reference_points,
+            spatial_shapes=spatial_shapes, level_start_index=level_start_index)[0])
+        return after(self.final_layer_norm, x, self.mlp(x))
