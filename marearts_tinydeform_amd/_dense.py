@@ -16,6 +16,7 @@ from ._native import DTYPE_CODES, INT32_MAX, _check, _ptr, _require, _stream, ac
 
 MAX_HEAD_DIM = 256        # TD_ATTN_MAX_HEAD_DIM
 MAX_NORM_CHANNELS = 16384  # TD_NORM_MAX_CHANNELS
+MAX_ATTN_ROWS = INT32_MAX - 1023
 MASK_NONE, MASK_BYTES, MASK_FLOAT = 0, 1, 2  # TD_MASK_*
 
 _i64, _vp, _int = ctypes.c_int64, ctypes.c_void_p, ctypes.c_int
@@ -78,7 +79,7 @@ def check_attn(query, key, value, attn_mask=None, key_padding_mask=None, scale=N
         raise RuntimeError('all float tensors must have the same dtype')
     if key.device != device or value.device != device:
         raise RuntimeError('all tensors must be on the same device')
-    if Q > INT32_MAX or K > INT32_MAX or B * Q * H > INT32_MAX or B * K * Hk > INT32_MAX:
+    if max(Q, K, B * Q * H, B * K * Hk) > MAX_ATTN_ROWS:
         raise RuntimeError('too many (batch, token, head) rows')
     if scale is None:
         scale = D ** -0.5

@@ -392,6 +392,7 @@ AttnParams attn_params(const td_attn_args& a) {
 namespace {
 
 constexpr int64_t kIntMax = 2147483647;
+constexpr int64_t kMaxRows = kIntMax - 1023;  // the numbers of a last tile's rows are 32-bit too
 
 int check_args(const td_attn_args* a) {
     set_error(TD_OK, "");
@@ -403,8 +404,8 @@ int check_args(const td_attn_args* a) {
         return set_error(TD_E_ARG, "the heads of key and value must divide the heads of query");
     if (a->D < 1 || a->D > TD_ATTN_MAX_HEAD_DIM)
         return set_error(TD_E_ARG, "head dim must be from 1 to %d", TD_ATTN_MAX_HEAD_DIM);
-    if (a->B > kIntMax || a->Q > kIntMax || a->K > kIntMax || a->H > kIntMax ||
-        static_cast<__int128>(a->B) * a->Q * a->H > kIntMax || static_cast<__int128>(a->B) * a->K * a->Hk > kIntMax)
+    if (a->B > kIntMax || a->Q > kMaxRows || a->K > kMaxRows ||
+        static_cast<__int128>(a->B) * a->Q * a->H > kMaxRows || static_cast<__int128>(a->B) * a->K * a->Hk > kMaxRows)
         return set_error(TD_E_ARG, "too many (batch, token, head) rows");
     for (int i = 0; i < 3; ++i)
         if (a->query_stride[i] < 0 || a->key_stride[i] < 0 || a->value_stride[i] < 0 || a->mask_stride[i] < 0)

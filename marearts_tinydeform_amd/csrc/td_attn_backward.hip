@@ -235,9 +235,9 @@ __global__ __launch_bounds__((kWaves<T, DP, WK> * kWave), (dq_min_waves<T, DP, W
     const float ds_scale = ds_factor<T>(p, info, bh, lane);
     const float delta = ri[2] * ds_scale;
     const T* const mrow = MASK ? static_cast<const T*>(p.mask) + b * p.ms[0] + h * p.ms[1] + i * p.ms[2] : nullptr;
-    // an additive mask may make m so large that log2 l is lost beside it: it is subtracted after t - m then
-    const bool apart = MASK && p.mask_type == TD_MASK_FLOAT;
-    const float from = apart ? ri[0] : ri[0] + ri[1] - kPShift<T>, then = apart ? ri[1] - kPShift<T> : 0.f;
+    // log2 l would be lost beside a large m (of large scores, or of an additive mask): it is subtracted after t - m then
+    const bool apart = __any(live && big_score(ri[0])) || (MASK && p.mask_type == TD_MASK_FLOAT);
+    const float from = (apart ? 0.f : ri[0]) + (ri[1] - kPShift<T>);
     const int diag = static_cast<int>(p.diag);
     const int last = p.causal ? i + diag : 2147483647;
     int kend = p.K;
@@ -332,13 +332,15 @@ __global__ __launch_bounds__((kWaves<T, DP, WK> * kWave), (dq_min_waves<T, DP, W
                                    bits[x] | static_cast<uint32_t>(gone >> (32 * x)) | beyond(j + 32 * x, last),
                                    values[x] ? mrow + j + 32 * x : nullptr, p.K - j - 32 * x, half);
                 }
+                if (apart) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[e] = rounded_product(s[e], cc) - ri[0];
+                    cc = 1.f;
+                }
                 f32x16 ds;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    float y = fmaf(s[e], cc, -from);
-                    if (apart) y -= then;
-                    ds[e] = __builtin_amdgcn_exp2f(y) * fmaf(dp[e], ds_scale, -delta);
-                }
+                for (int e = 0; e < 16; ++e)
+                    ds[e] = __builtin_amdgcn_exp2f(fmaf(s[e], cc, -from)) * fmaf(dp[e], ds_scale, -delta);
                 typename R::Packed w[R::kPacked];
                 R::pack(ds, w);
 #pragma unroll
@@ -401,7 +403,7 @@ constexpr int dkv_row_tile() {
     return WK || DP * static_cast<int>(sizeof(T)) > 128 ? 32 : 64;
 }
 
-// What LDS holds of a row beside its elements: m, log2 l, delta, the mask words of the workgroup's keys, and with a mask
+// What LDS holds of a row beside its elements: m + log2 l (or log2 l, and m apart from it), delta, the mask words of the workgroup's keys, and with a mask
 // its kind for each word and the row's offset in it
 template <typename T, int DP, bool WK>
 constexpr bool v_in_lds() {
@@ -433,8 +435,8 @@ __global__ __launch_bounds__((kWaves<T, DP, WK> * kWave), (dkv_min_waves<T, DP, 
     unsigned char* const q_lds = lds + (WK ? wave * kArea : 0);
     unsigned char* const g_lds = q_lds + kTile;
     float* const m_lds = reinterpret_cast<float*>(g_lds + kTile);
-    float* const l_lds = m_lds + RT;
-    float* const d_lds = l_lds + RT;
+    float* const a_lds = m_lds + RT;
+    float* const d_lds = a_lds + RT;
     uint32_t* const w_lds = reinterpret_cast<uint32_t*>(d_lds + RT);   // [KW][RT]
     int* const k_lds = reinterpret_cast<int*>(w_lds + KW * RT);        // [KW][RT], with a mask
     int64_t* const o_lds = reinterpret_cast<int64_t*>(k_lds + KW * RT);
@@ -541,8 +543,9 @@ __global__ __launch_bounds__((kWaves<T, DP, WK> * kWave), (dkv_min_waves<T, DP, 
         if (!WK) __syncthreads();
         staged.store(q_lds, g_lds, p.D);
         if (t < RT) {
-            m_lds[t] = apart ? ri[0] : ri[0] + ri[1] - kPShift<T>;
-            l_lds[t] = ri[1] - kPShift<T>;
+            const bool two = ri[0] < __builtin_inff() && (apart || big_score(ri[0]));
+            m_lds[t] = (two ? 0.f : ri[0]) + (ri[1] - kPShift<T>);
+            a_lds[t] = two ? ri[0] : 0.f;
             d_lds[t] = ri[2] * ds_scale;
             if (MASK) o_lds[t] = mo;
             if (bits) {
@@ -599,19 +602,24 @@ __global__ __launch_bounds__((kWaves<T, DP, WK> * kWave), (dkv_min_waves<T, DP, 
                         }
                     }
                 }
+                if (apart || __any(a_lds[32 * x + (lane & 31)] != 0.f)) {
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        const f32x4 a4 = *reinterpret_cast<const f32x4*>(a_lds + 32 * x + 8 * y + 4 * half);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[4 * y + e] = rounded_product(s[4 * y + e], cc) - a4[e];
+                    }
+                    cc = 1.f;
+                }
                 f32x16 ds;
 #pragma unroll
                 for (int y = 0; y < 4; ++y) {
                     const int row = 32 * x + 8 * y + 4 * half;
                     const f32x4 m4 = *reinterpret_cast<const f32x4*>(m_lds + row);
                     const f32x4 d4 = *reinterpret_cast<const f32x4*>(d_lds + row);
-                    f32x4 l4 = f32x4{0.f, 0.f, 0.f, 0.f};
-                    if (apart) l4 = *reinterpret_cast<const f32x4*>(l_lds + row);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        float z = fmaf(s[4 * y + e], cc, -m4[e]);
-                        if (apart) z -= l4[e];
-                        const float pr = __builtin_amdgcn_exp2f(z);
+                        const float pr = __builtin_amdgcn_exp2f(fmaf(s[4 * y + e], cc, -m4[e]));
                         s[4 * y + e] = pr;
                         ds[4 * y + e] = pr * fmaf(dp[4 * y + e], ds_scale, -d4[e]);
                     }

@@ -21,6 +21,11 @@ constexpr float kSlack = 4.f;
 // steps of 2^-35. The factor is in l as well and cancels.
 template <typename T>
 constexpr float kShift = std::is_same<T, f16>::value ? 11.f : 0.f;
+// log2 of the factor that l holds: 11 as far as m has bits for it
+template <typename T>
+__device__ __forceinline__ float shift_of(float m) {
+    return kShift<T> == 0.f ? 0.f : m - (m - kShift<T>);
+}
 
 struct Split {
     TileSplit t;
@@ -109,6 +114,7 @@ __global__ __launch_bounds__((kWaves<T, DP, WK> * kWave), (min_waves<T, DP, WK, 
     auto v_row = [&](int x) { return x * p.vs[1]; };
     staged.plan(k_row, v_row, p.D);
     float m = kNegInf, l = 0.f;
+    bool big = false;  // a row's maximum is
     f32x16 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = f32x16{0.f};
@@ -179,9 +185,17 @@ __global__ __launch_bounds__((kWaves<T, DP, WK> * kWave), (min_waves<T, DP, WK, 
                 const float to = __builtin_fmaxf(m, mt);
                 const float shrink = to == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m - to);
                 m = to;
+                big = __any(big_score(m));
                 l *= shrink;
 #pragma unroll
                 for (int d = 0; d < ND; ++d) o[d] *= shrink;
+            }
+            if (big) {
+#pragma unroll
+                for (int x = 0; x < KT / 32; ++x)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[x][e] = rounded_product(s[x][e], cc);
+                cc = 1.f;
             }
             const float from = m == kNegInf ? 0.f : m - kShift<T>;
 #pragma unroll
@@ -289,7 +303,7 @@ __global__ __launch_bounds__((kWaves<T, DP, WK> * kWave), (min_waves<T, DP, WK, 
     if (p.stats != nullptr && half == 0) {
         float* const st = static_cast<float*>(p.stats) + 2 * row;
         st[0] = l == 0.f ? 0.f : m;
-        st[1] = l == 0.f ? 0.f : __builtin_amdgcn_logf(l) - kShift<T>;
+        st[1] = l == 0.f ? 0.f : __builtin_amdgcn_logf(l) - shift_of<T>(m);
     }
 }
 
@@ -362,7 +376,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p, Split sp, 
     if (p.stats != nullptr && x == 0) {
         float* const st = static_cast<float*>(p.stats) + 2 * ((static_cast<int64_t>(b) * p.H + h) * p.Q + i);
         st[0] = l == 0.f ? 0.f : m;
-        st[1] = l == 0.f ? 0.f : __builtin_amdgcn_logf(l) - kShift<T>;
+        st[1] = l == 0.f ? 0.f : __builtin_amdgcn_logf(l) - shift_of<T>(m);
     }
 }
 

@@ -301,6 +301,17 @@ __device__ __forceinline__ float mask_log2(float m) {
     return m == kNegInf ? kNegInf : __builtin_fmaxf(m * kLog2e, kLowest);
 }
 
+// Scores past 2^16 (base 2) have steps of 2^-8 or more: fma(score, c, -m), which does not round the product, no longer
+// cancels against a maximum m that was a rounded product, and what is added to m (log2 l, a factor's exponent) loses its
+// bits. Rows of such a maximum take the products rounded and add the rest to the difference.
+__device__ __forceinline__ bool big_score(float m) {
+    return __builtin_fabsf(m) > 65536.f && __builtin_fabsf(m) < __builtin_inff();
+}
+__device__ __forceinline__ float rounded_product(float s, float c) {
+#pragma clang fp contract(off)
+    return s * c;
+}
+
 // Keys j0 .. j0 + 31 beyond `last`, the last key that a query sees, as bits
 __device__ __forceinline__ uint32_t beyond(int j0, int last) {
     return last < j0 ? ~0u : last - j0 >= 31 ? 0u : ~0u << (last - j0 + 1);

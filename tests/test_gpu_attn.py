@@ -160,6 +160,49 @@ def test_large_scores(dtype):
     check_attn(dtype, q, k, v, go, {}, out, grads)
 
 
+@pytest.mark.parametrize('size', [(1, 60, 130), (2, 8400, 130), (1, 3, 4100)])
+@pytest.mark.parametrize('masked', [False, True])
+@pytest.mark.parametrize('dtype', TYPES)
+def test_scores_past_the_bits_of_their_logarithm(dtype, masked, size):
+    """Scores of 2^25 and more, whose float32 steps are larger than log2 of the row's sum: ten patterns of signs as queries
+    and keys, so that each query attends evenly to the keys of its own pattern and every score is exact.
+
+    The bounds: an even probability is exact before it is divided; rounded to the type (half a step u) in the backward
+    pass, as dS is, and every result is rounded once. grad_out . out holds u^2 of its terms (out with its remainder), sums
+    in float32 64 half steps of theirs."""
+    B, Q, K = size
+    g = torch.Generator().manual_seed(5)
+    signs = torch.randint(0, 2, (10, 32), generator=g).double() * 4096 - 2048
+    q = signs[torch.arange(Q) % 10][None, :, None].expand(B, -1, -1, -1).to(dtype)
+    k = signs[torch.arange(K) % 10][None, :, None].expand(B, -1, -1, -1).to(dtype)
+    v = torch.randn(B, K, 1, 32, generator=g).to(dtype)
+    go = torch.randn(B, Q, 32, generator=g).to(dtype)
+    go[:, 100:] = 0  # so that sums over thousands of queries stay within float16
+    kw = {}
+    if masked:
+        kw['key_padding_mask'] = torch.zeros(B, K, dtype=torch.bool)
+        kw['key_padding_mask'][:, -3:] = True
+    out, grads = run(q, k, v, go, kw)
+    out, (dq, dk, dv) = out.detach().double().cpu()[:, :100], [t.double().cpu()[:, :, 0] for t in grads]
+    q, k, v, go = q.double()[:, :100, 0], k.double()[:, :, 0], v.double()[:, :, 0], go.double()[:, :100]
+    live = torch.ones(B, K) if not masked else (~kw['key_padding_mask']).double()
+    P = (torch.arange(q.size(1))[:, None] % 10 == torch.arange(K)[None] % 10).double() * live[:, None]
+    P = P / P.sum(-1, keepdim=True)
+    o = P @ v
+    scale, u, f = 32 ** -0.5, torch.finfo(dtype).eps / 2, 2.0 ** -24
+    dp, delta = go @ v.transpose(1, 2), (go * o).sum(-1, keepdim=True)
+    ds = P * (dp - delta)
+    e_ds = 2 * u * ds.abs() + P * (u * u + 64 * f) * (go.abs() @ v.abs().transpose(1, 2) +
+                                                      (go * o).abs().sum(-1, keepdim=True))
+    for name, got, want, bound in (
+            ('out', out, o, 64 * f * (P @ v.abs())), ('dv', dv, P.transpose(1, 2) @ go, (u + 64 * f) * (P.transpose(1, 2) @ go.abs())),
+            ('dq', dq[:, :100], ds @ k * scale, e_ds @ k.abs() * scale),
+            ('dk', dk, ds.transpose(1, 2) @ q * scale, e_ds.transpose(1, 2) @ q.abs() * scale)):
+        excess = (got - want).abs() - bound - u * want.abs() - 2.0 ** -24
+        assert float(excess.max()) <= 0, f'{name}: {float(excess.max()):.3g} past its bound'
+        assert torch.isfinite(got).all(), name
+
+
 @pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
 def test_small_and_large_gradients(dtype):
     # gradients of a loss over many tokens (1e-4) and of a scaled loss (1e3): dS is rounded to 16 bits
