@@ -39,7 +39,7 @@ typedef struct td_attn_args {
     int32_t mask_type; /* TD_MASK_* */
     int32_t causal;
     int32_t reserved; /* 0 */
-    int64_t B, Q, K, H, Hk, D; /* Hk divides H; D <= TD_ATTN_MAX_HEAD_DIM; Q, K, B * Q * H, B * K * Hk <= INT32_MAX */
+    int64_t B, Q, K, H, Hk, D; /* Hk divides H; D <= TD_ATTN_MAX_HEAD_DIM; Q, K, B * Q * H, B * K * Hk <= INT32_MAX - 1023 */
     double scale;              /* finite, > 0 */
     const void* query;         /* [B, Q, H, D], element strides below (batch, token, head; not negative), the last one 1 */
     const void* key;           /* [B, K, Hk, D] */

@@ -291,10 +291,18 @@ __global__ __launch_bounds__(256) void attn_mask_kernel(AttnParams p, int64_t ti
             }
         } else {
             const T* m = static_cast<const T*>(p.mask) + m0;
-            for (int k = 0; k < 32 && k < left; ++k) {
-                const float v = static_cast<float>(m[k]);
+            auto see = [&](T entry, int k) {
+                const float v = static_cast<float>(entry);
                 if (v != neg_inf<float>()) bits &= ~(1u << k);
                 values |= v != 0.f && v != neg_inf<float>();
+            };
+            if (left >= 32) {
+                T v[32];
+                __builtin_memcpy(v, m, sizeof(v));
+#pragma unroll
+                for (int k = 0; k < 32; ++k) see(v[k], k);
+            } else {
+                for (int k = 0; k < left; ++k) see(m[k], k);
             }
         }
         p.bits[(at * mask_rows + row) * p.words + word] = bits;

@@ -355,10 +355,16 @@ __device__ __forceinline__ void mask_scores(f32x16& s, float c, uint32_t gone, c
     for (int i = 0; i < 4; ++i) {
         float add[4] = {0.f, 0.f, 0.f, 0.f};
         if (values != nullptr) {
+            const int key = 8 * i + 4 * half;
+            if (key + 4 <= left) {
+                T four[4];  // no alignment is known, the hardware needs none
+                __builtin_memcpy(four, values + key, sizeof(four));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int key = 8 * i + 4 * half + e;
-                if (key < left) add[e] = mask_log2(static_cast<float>(values[key]));
+                for (int e = 0; e < 4; ++e) add[e] = mask_log2(static_cast<float>(four[e]));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (key + e < left) add[e] = mask_log2(static_cast<float>(values[key + e]));
             }
             __builtin_amdgcn_sched_barrier(0);  // four loads at a time: registers
         }
