@@ -572,6 +572,15 @@ __global__ __launch_bounds__((kWaves<T, DP, WK> * kWave), (dkv_min_waves<T, DP, 
                     masked |= __any(kind != kMaskNone);
                     values = __any(kind == kMaskValues);
                 }
+                // the mask's values at the lane's key, on their way during the products where registers are left for them
+                constexpr bool kEarly = MASK && DP * sizeof(T) <= 128;
+                T entries[kEarly ? 16 : 1];
+                if constexpr (kEarly)
+                    if (values)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            entries[e] = static_cast<const T*>(
+                                p.mask)[o_lds[32 * x + 8 * (e >> 2) + 4 * half + (e & 3)] + mask_key];
                 f32x16 s = f32x16{0.f}, dp = f32x16{0.f};
 #pragma unroll
                 for (int c = 0; c < R::kChunks; ++c) {
@@ -587,7 +596,11 @@ __global__ __launch_bounds__((kWaves<T, DP, WK> * kWave), (dkv_min_waves<T, DP, 
                         const int row = 32 * x + 8 * y + 4 * half;
                         const u32x4 w4 = *reinterpret_cast<const u32x4*>(my_words + row);
                         float add[4] = {0.f, 0.f, 0.f, 0.f};
-                        if (MASK && values) {
+                        if (kEarly && values) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                add[e] = mask_log2(static_cast<float>(entries[kEarly ? 4 * y + e : 0]));
+                        } else if (MASK && values) {
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
                                 add[e] = mask_log2(
