@@ -5,7 +5,8 @@
  * The conventions of tinydeform.h hold: plain device pointers, int64 sizes, a hipStream_t passed as void*; the library
  * never allocates, frees or synchronises, callers own every buffer (workspaces included), each call may be captured in
  * a HIP graph; TD_OK or a negative TD_E* code is returned, with td_last_error() describing the failure. dtype is TD_F32,
- * TD_F16, TD_BF16 or TD_F64; outputs do not overlap inputs; sums, softmax statistics and norms are float32 (float64 for TD_F64).
+ * TD_F16, TD_BF16 or TD_F64; outputs do not overlap inputs; sums, softmax statistics and norms are float32 (float64 for
+ * TD_F64).
  * No counterpart in the reference, whose operator is deformable attention alone.
  */
 #ifndef TINYDEFORM_DENSE_H
@@ -39,7 +40,8 @@ typedef struct td_attn_args {
     int32_t mask_type; /* TD_MASK_* */
     int32_t causal;
     int32_t reserved; /* 0 */
-    int64_t B, Q, K, H, Hk, D; /* Hk divides H; D <= TD_ATTN_MAX_HEAD_DIM; Q, K, B * Q * H, B * K * Hk <= INT32_MAX - 1023 */
+    /* Hk divides H; D <= TD_ATTN_MAX_HEAD_DIM; Q, K, B * Q * H, B * K * Hk <= INT32_MAX - 1023 */
+    int64_t B, Q, K, H, Hk, D;
     double scale;              /* finite, > 0 */
     const void* query;         /* [B, Q, H, D], element strides below (batch, token, head; not negative), the last one 1 */
     const void* key;           /* [B, K, Hk, D] */
@@ -54,14 +56,16 @@ typedef struct td_attn_args {
                                    grad_out . out then has twice the bits. Or NULL */
 } td_attn_args;
 
-/* Bytes of workspace td_attn_forward needs (0 for many problems; a mask takes an eighth of a byte a pair), or a negative TD_E* code. No memory is read. */
+/* Bytes of workspace td_attn_forward needs (0 for many problems; a mask takes an eighth of a byte an entry), or a negative
+ * TD_E* code. No memory is read. */
 int64_t td_attn_forward_workspace(const td_attn_args* args);
 int td_attn_forward(const td_attn_args* args, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Gradients of td_attn_forward, the probabilities computed again from the scores and `stats`. args: as in the forward
- * call, with the out, stats and out_low (or NULL) that it wrote. grad_out [B, Q, H * D], grad_query [B, Q, H, D], grad_key and grad_value
- * [B, K, Hk, D] are contiguous, in dtype; grad_query, or grad_key and grad_value together, may be NULL (not computed).
+ * call, with the out, stats and out_low (or NULL) that it wrote. grad_out [B, Q, H * D], grad_query [B, Q, H, D],
+ * grad_key and grad_value [B, K, Hk, D] are contiguous, in dtype; grad_query, or grad_key and grad_value together, may be
+ * NULL (not computed).
  * No atomics: the results are the same on every run.
  */
 int64_t td_attn_backward_workspace(const td_attn_args* args);

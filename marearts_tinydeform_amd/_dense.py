@@ -149,7 +149,7 @@ def attn_forward(query, key, value, attn_mask=None, key_padding_mask=None, scale
     if train:
         stats = torch.empty((B, H, Q, 2), dtype=acc_dtype(dtype), device=dev)
         if dtype in (torch.float16, torch.bfloat16):  # what rounding took from out: grad_out . out needs it
-            low = torch.empty((B, Q, H * D), dtype=dtype, device=dev)
+            low = torch.empty_like(out)
     if B * Q > 0:
         args = _pack(q, k, v, mask, kind, strides, pad, scale, causal, out, stats, low)
         need = lib.td_attn_forward_workspace(args)
@@ -168,12 +168,12 @@ def attn_backward(tensors, values, grad_out, need_query=True, need_key_value=Tru
     kind, strides, scale, causal = values
     if grad_out.shape != out.shape or grad_out.dtype != q.dtype or grad_out.device != q.device:
         raise RuntimeError('grad_out must be [B, Q, H * D] like the forward output')
-    dev, dtype, go = q.device, q.dtype, grad_out.contiguous()
-    dq = torch.empty(q.shape, dtype=dtype, device=dev) if need_query else None
+    dev, go = q.device, grad_out.contiguous()
+    dq = torch.empty_like(q, memory_format=torch.contiguous_format) if need_query else None
     dk = dv = None
     if need_key_value:
-        dk = torch.empty(k.shape, dtype=dtype, device=dev)
-        dv = torch.empty(k.shape, dtype=dtype, device=dev)
+        dk = torch.empty_like(k, memory_format=torch.contiguous_format)
+        dv = torch.empty_like(k, memory_format=torch.contiguous_format)
     if q.size(0) * (q.size(1) + k.size(1)) > 0:
         args = _pack(q, k, v, mask, kind, strides, pad, scale, causal, out, stats, low)
         need = lib.td_attn_backward_workspace(args)
@@ -223,7 +223,7 @@ def layer_norm_forward(x, weight, bias, residual=None, eps=1e-5, train=False):
         raise RuntimeError('eps must be non-negative and finite')
     dev = x.device
     x, weight, bias, residual = x.contiguous(), _contiguous(weight), _contiguous(bias), _contiguous(residual)
-    out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    out = torch.empty_like(x)
     stats = torch.empty((rows, 2), dtype=acc_dtype(x.dtype), device=dev) if train else None
     if rows > 0:
         _check(lib.td_layer_norm_forward(DTYPE_CODES[x.dtype], x.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias),
@@ -241,7 +241,7 @@ def layer_norm_backward(tensors, grad_out, need_weight=True, need_bias=True):
     rows, C = stats.size(0), x.size(-1)
     dev, dtype, go = x.device, x.dtype, grad_out.contiguous()
     code = DTYPE_CODES[dtype]
-    dx = torch.empty(x.shape, dtype=dtype, device=dev)
+    dx = torch.empty_like(x)
     dw = torch.empty((C,), dtype=dtype, device=dev) if need_weight else None
     db = torch.empty((C,), dtype=dtype, device=dev) if need_bias else None
     need = lib.td_layer_norm_backward_workspace(code, rows, C) if need_weight or need_bias else 0

@@ -3,8 +3,16 @@
 //   dV = P^T g,  dP = g V^T,  dS = P (dP - delta),  delta = g . out,  dQ = scale dS K,  dK = scale dS^T Q.
 // Three launches: delta (and the statistics in the order of the problem's rows); dQ, a workgroup's rows against every key,
 // as the forward; dK and dV, a workgroup's keys against every row, so that no sum needs an atomic. That computes scores
-// and dP twice, 7 products where 5 would do; the other way, dQ summed over key blocks in memory, moves 4 D bytes for each
-// 32 D flops of a 128-key block's pairs and rows.
+// and dP twice, 7 products where 5 would do; the other way, dQ summed over key blocks in memory, moves 8 D bytes (read and
+// written) for each row and block of 256 keys, and its order or its atomics change the result.
+//
+// P and dS are rounded to the inputs' type for their products: half a step of each, which leaves dQ and dK of 16-bit inputs
+// with 1.4 to 1.5 times the error of one rounding at the end (a second, low part of dS would take that out for another
+// product).
+//
+// Bound by the vector units where heads are narrow, by LDS reads beside the MFMAs where they are wide: 8400 tokens x 8
+// heads of 32, float16, batch 2: dQ 320 us (680 TFLOP/s), dK and dV 410 (700); 4096 x 16 heads of 64, bfloat16: 240 (860)
+// and 316 (870); of 128: 435 (950) and 688 (800).
 #include "td_attn_mma.h"
 
 #ifndef TD_ATTN_TYPE
@@ -132,6 +140,8 @@ constexpr int dq_key_tile() {
     return WK || DP * static_cast<int>(sizeof(T)) > 128 ? 32 : 64;
 }
 // Wavefronts a SIMD that the registers leave room for with few spills or none. A workgroup of eight takes two of each SIMD.
+// dK and dV under a mask (SLOW) stay at two: at four they spill 90 to 120 registers (1100 x 64 heads of 32, bfloat16: 87
+// us, 182 with the spills).
 template <typename T, int DP, bool WK, bool SLOW>
 constexpr int dq_min_waves() {
     constexpr int bytes = DP * static_cast<int>(sizeof(T));
@@ -200,9 +210,8 @@ void sum_parts(const AttnParams& p, const TileSplit& t, const float* part, void*
                        part, static_cast<T*>(out), quads, tile_rows, tiles, keys, p.D % 4 == 0);
 }
 template <typename T, int DP, bool WK, bool MASK, bool VEC>
-__global__ __launch_bounds__((kWaves<T, DP, WK> * kWave), (dq_min_waves<T, DP, WK, MASK>())) void attn_dq_kernel(AttnParams p, RowInfo info,
-                                                                                    Parts parts, bool vec_out,
-                                                                                    int tiles) {
+__global__ __launch_bounds__((kWaves<T, DP, WK> * kWave), (dq_min_waves<T, DP, WK, MASK>())) void attn_dq_kernel(
+    AttnParams p, RowInfo info, Parts parts, bool vec_out, int tiles) {
     using R = TileRows<T, DP>;
     constexpr int KT = dq_key_tile<T, DP, WK>(), ND = DP / 32, BM = kTileRows<T, DP, WK>;
     constexpr int kTile = KT * R::kPitch;
@@ -396,19 +405,20 @@ __global__ __launch_bounds__((kWaves<T, DP, WK> * kWave), (dq_min_waves<T, DP, W
         }
 }
 
-// dK and dV. WK: private row tiles. The scores stand untransposed here (a lane's column is its key), so that P and dS are operands
-// of dV^T = g^T P and dK^T = Q^T dS as they stand. Rows past the end hold zeros and m = inf: P = 0.
+// dK and dV. WK: private row tiles. The scores stand untransposed here (a lane's column is its key), so that P and dS are
+// operands of dV^T = g^T P and dK^T = Q^T dS as they stand. Rows past the end hold zeros and m = inf: P = 0.
 template <typename T, int DP, bool WK>
 constexpr int dkv_row_tile() {
     return WK || DP * static_cast<int>(sizeof(T)) > 128 ? 32 : 64;
 }
 
-// What LDS holds of a row beside its elements: m + log2 l (or log2 l, and m apart from it), delta, the mask words of the workgroup's keys, and with a mask
-// its kind for each word and the row's offset in it
+// V of wide heads stays in LDS: its fragments would spill. With dK and dV the registers hold K's fragments only.
 template <typename T, int DP, bool WK>
 constexpr bool v_in_lds() {
     return !WK && DP * static_cast<int>(sizeof(T)) == 256;
 }
+// What LDS holds of a row beside its elements: m + log2 l (or log2 l, and m apart from it), delta, the mask words of the
+// workgroup's keys, and with a mask its kind for each word and the row's offset in it
 template <typename T, int DP, bool WK, bool MASK>
 constexpr int dkv_row_bytes() {
     constexpr int words = kTileRows<T, DP, WK> / 8;  // bytes
@@ -416,9 +426,8 @@ constexpr int dkv_row_bytes() {
 }
 
 template <typename T, int DP, bool WK, bool MASK, bool VEC>
-__global__ __launch_bounds__((kWaves<T, DP, WK> * kWave), (dkv_min_waves<T, DP, WK, MASK>())) void attn_dkv_kernel(AttnParams p, RowInfo info,
-                                                                                     Parts parts, bool vec_out,
-                                                                                     int tiles) {
+__global__ __launch_bounds__((kWaves<T, DP, WK> * kWave), (dkv_min_waves<T, DP, WK, MASK>())) void attn_dkv_kernel(
+    AttnParams p, RowInfo info, Parts parts, bool vec_out, int tiles) {
     using R = TileRows<T, DP>;
     constexpr int RT = dkv_row_tile<T, DP, WK>(), ND = DP / 32, BM = kTileRows<T, DP, WK>;
     constexpr int kTile = RT * R::kPitch;
@@ -727,10 +736,14 @@ bool back_vec(int dtype, const AttnParams& p) {
            static_cast<int64_t>(p.H) * p.D < (int64_t{1} << 31) / (128 * elem);
 }
 
-// Workgroups of 256 rows (keys) that share tiles, when they fill the GPU; else of 32 rows (keys) with the others'
-// tiles over the wavefronts, which needs no second launch, for heads whose private tiles fit in the registers. Where that
+// Workgroups of 256 rows (keys) that share tiles, when they fill the GPU; else of 32 rows (keys) with the others' tiles
+// over the wavefronts, which needs no second launch, for heads whose private tiles fit in the registers. Where that
 // still leaves CUs without work and the loops are long, parts; where many tiles leave a few over, parts of those
-// (even_split).
+// (even_split). Measured, both sides: private below 384 x 128 rows (4 key heads x 16000 rows of 64, bfloat16, 500: dQ 170
+// us, shared 143; 2 x 12 heads x 1500, 288: 53, shared 60, dK and dV 67, shared 86), but not for long loops (2 x 8 x 1000 of
+// 32 over 12000 keys: dQ 87, shared 68); a part has 256 steps or more of a shared tile (8 heads x 1500 of 128: dQ 58 us with
+// 512, 44 with 256, dK and dV 87 and 64), 1024 of a private one (3000 rows by 2 x 8 x 200 keys of 64: 33 us, with 512 39,
+// with 256 45); parts below 256 shared workgroups (64 heads x 1100 as 320: dQ 45 us, in parts 52).
 BackShape back_shape(int dtype, const AttnParams& p, bool vec) {
     BackShape s{};
     s.vec = vec;
@@ -738,14 +751,15 @@ BackShape back_shape(int dtype, const AttnParams& p, bool vec) {
     const bool can = vec && padded_width(p.D) * elem_size(dtype) <= 128;
     auto shape = [&](int n, int over) {
         BackShape::One o{};
-        o.wk = can && heads * ((n + 127) / 128) < 512;
+        const bool long_loop = over >= 8192 && n >= 512;
+        o.wk = can && !long_loop && heads * ((n + 127) / 128) < 384;
         o.tile_rows = tile_rows(o.wk, padded_width(p.D) * elem_size(dtype));
         o.tiles = (n + o.tile_rows - 1) / o.tile_rows;
         const int total = static_cast<int>(heads * o.tiles);
         o.t = TileSplit{1, total, total};
         const int few = o.tile_rows == 256 ? 256 : 384;
         if (total > 0 && total < few) {
-            const int want = ((o.tile_rows == 256 ? 512 : 1024) + total - 1) / total, most = over / 512;  // 4 steps of 4 x 32 or 16 of 32 a part
+            const int want = ((o.tile_rows == 256 ? 512 : 1024) + total - 1) / total, most = over / (o.wk ? 1024 : 256);
             const int parts = want < most ? want : most;
             if (parts > 1) o.t = TileSplit{parts, 0, total};
         } else if (!o.wk && !p.causal) {
@@ -780,7 +794,8 @@ int run_dq(const AttnParams& p, const BackShape& s, const RowInfo& info, float* 
 template <typename T, int DP, bool WK, bool MASK, bool VEC>
 int run_dkv(const AttnParams& p, const BackShape& s, const RowInfo& info, float* ws, hipStream_t stream) {
     static std::atomic<uint64_t> done{0};
-    constexpr int RT = dkv_row_tile<T, DP, WK>(), area = 2 * RT * TileRows<T, DP>::kPitch + RT * dkv_row_bytes<T, DP, WK, MASK>();
+    constexpr int RT = dkv_row_tile<T, DP, WK>();
+    constexpr int area = 2 * RT * TileRows<T, DP>::kPitch + RT * dkv_row_bytes<T, DP, WK, MASK>();
     constexpr int join = 2 * 32 * (DP + 4) * 4;
     constexpr int own = v_in_lds<T, DP, WK>() ? kTileRows<T, DP, WK> * TileRows<T, DP>::kPitch : 0;
     constexpr int bytes = WK ? (4 * area > join ? 4 * area : join) : area + own;

@@ -3,7 +3,14 @@
 // One pass over the keys with the running maximum m and sum l of the softmax (Milakov and Gimelshein, "Online normalizer
 // calculation for softmax", 2018): S^T = K Q^T, P^T = 2^(S^T - m), O^T += V^T P^T, all three transposed, so that a
 // lane's scores are of one row (its column), the row's statistics are one number a lane, and P^T is the second product's
-// operand as it stands in the accumulator.
+// operand as it stands in the accumulator. P is rounded to the inputs' type for that product (half a step of each, not
+// summed up: l adds the unrounded ones); everything else stays in float32.
+//
+// Bound by the vector units where heads are narrow: a score costs an exponential and five operations beside D / 32 of an
+// MFMA's work (8400 tokens x 8 heads of 32, float16, batch 2: 243 to 264 us, 230 of them vector operations, MFMA busy 24%);
+// by LDS reads and MFMAs together where they are wide (4096 tokens x 16 heads, bfloat16, batch 2: 64 wide 165 us, 830
+// TFLOP/s, 128 wide 311 us, 883); by memory for single tokens (4 x 21760 keys, 4 key heads of 64: 18 us, 5 TB/s, and 6.7
+// for the join).
 #include "td_attn_mma.h"
 
 // The build compiles this file once per type: TD_ATTN_TYPE 0 float32 (and the entry), 1 float16, 2 bfloat16.
@@ -51,8 +58,8 @@ constexpr int min_waves() {
 // WK: private key tiles (TwoTiles); the four wavefronts' partial results are joined in LDS.
 // MASK: there is a mask tensor. VEC: operands are read 16 bytes at a time (StagedRows).
 template <typename T, int DP, bool WK, bool MASK, bool VEC>
-__global__ __launch_bounds__((kWaves<T, DP, WK> * kWave), (min_waves<T, DP, WK, MASK>())) void attn_forward_kernel(AttnParams p, Split sp, bool vec_out,
-                                                                               int tiles) {
+__global__ __launch_bounds__((kWaves<T, DP, WK> * kWave), (min_waves<T, DP, WK, MASK>())) void attn_forward_kernel(
+    AttnParams p, Split sp, bool vec_out, int tiles) {
     using R = TileRows<T, DP>;
     constexpr int KT = key_tile<T, DP, WK>(), ND = DP / 32, BM = kTileRows<T, DP, WK>;
     constexpr int kTile = KT * R::kPitch;
@@ -381,8 +388,12 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p, Split sp, 
 }
 
 // The launch shape. Workgroups of 256 rows that share key tiles, when they fill the GPU, with what is left over after an
-// even share for every CU split (even_split); else workgroups of 32 rows with the keys over the wavefronts, and when
-// those are few and the keys many, the keys over several workgroups too.
+// even share for every CU split (even_split); else workgroups of 32 rows with the keys over the wavefronts. Where either
+// leaves CUs without work and the keys are many, the keys are split over workgroups too. Measured, both sides of each rule:
+// private tiles below 512 x 128 rows (2 x 12 heads x 1500 of 64, bfloat16: 39 us, shared 53; 3 x 8 x 1100 of 32: 19, 34),
+// but not for long loops of enough rows (2 x 8 x 1000 of 32 over 12000 keys: 87, shared in 8 parts 62; 8 heads x 100 over
+// 8000: 21, shared 26). Parts below 256 workgroups (8 heads x 2000 as 504 private ones: 20 us whole, 28 in parts; 64 heads x
+// 1100 as 320 shared ones: 38 whole, 62 in parts).
 struct Shape {
     bool vec, wk;
     int tile_rows, tiles, keys;
@@ -399,14 +410,15 @@ Shape shape_of(int dtype, const AttnParams& p) {
     s.vec = p.D * elem % 16 == 0 && ok(p.q, p.qs) && ok(p.k, p.ks) && ok(p.v, p.vs);
     const int64_t heads = static_cast<int64_t>(p.B) * p.Hk;
     const bool can = s.vec && padded_width(p.D) * elem <= 256;  // wider rows' private tiles do not fit in registers
-    s.wk = can && heads * ((p.rows + 127) / 128) < 512;
+    const bool long_loop = p.K >= 8192 && p.rows >= 512;
+    s.wk = can && !long_loop && heads * ((p.rows + 127) / 128) < 512;
     s.tile_rows = tile_rows(s.wk, padded_width(p.D) * elem);
     s.tiles = (p.rows + s.tile_rows - 1) / s.tile_rows;
     const int total = static_cast<int>(heads * s.tiles);
     s.t = TileSplit{1, total, total};
-    const int few = s.tile_rows == 256 ? 256 : 512;  // workgroups that a CU's worth of work takes
-    if (total < few && p.K > 1024) {
-        int64_t n = (2 * few + total - 1) / total;
+    const bool big = s.tile_rows == 256;                  // of 512 threads: two such workgroups fill a CU
+    if (total < (big || s.wk ? 256 : 512) && p.K > 1024) {
+        int64_t n = ((big ? 512 : 1024) + total - 1) / total;
         const int64_t most = (p.K + 511) / 512;
         n = n < most ? n : most;
         n = n < kJoinParts ? n : kJoinParts;

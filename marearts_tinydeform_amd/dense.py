@@ -19,6 +19,16 @@ def _on_device(t, fn, *args):
         return fn(*args)
 
 
+def _once(backward):
+    """A backward pass that can be run once: once_differentiable refuses a second derivative, but costs 5 us of host time
+    that a step without one need not wait for."""
+    once = once_differentiable(backward)
+
+    def run(ctx, grad_out):
+        return once(ctx, grad_out) if torch.is_grad_enabled() else backward(ctx, grad_out)
+    return run
+
+
 def ma_attn(query, key, value, attn_mask=None, key_padding_mask=None, scale=None, causal=False):
     """Attention among tokens: softmax(scale * query key^T + mask) value for each head; [B, Q, H * D].
 
@@ -57,7 +67,7 @@ class _AttnFunction(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_out):
         need = ctx.needs_input_grad
         dq, dk, dv = _dense.attn_backward(ctx.saved_tensors, ctx.values, grad_out, need[0], need[1] or need[2])
@@ -104,7 +114,7 @@ class _LayerNormFunction(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_out):
         need = ctx.needs_input_grad
         dx, dw, db = _dense.layer_norm_backward(ctx.saved_tensors, grad_out, need[1], need[2])

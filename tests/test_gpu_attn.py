@@ -195,7 +195,8 @@ def test_scores_past_the_bits_of_their_logarithm(dtype, masked, size):
     e_ds = 2 * u * ds.abs() + P * (u * u + 64 * f) * (go.abs() @ v.abs().transpose(1, 2) +
                                                       (go * o).abs().sum(-1, keepdim=True))
     for name, got, want, bound in (
-            ('out', out, o, 64 * f * (P @ v.abs())), ('dv', dv, P.transpose(1, 2) @ go, (u + 64 * f) * (P.transpose(1, 2) @ go.abs())),
+            ('out', out, o, 64 * f * (P @ v.abs())),
+            ('dv', dv, P.transpose(1, 2) @ go, (u + 64 * f) * (P.transpose(1, 2) @ go.abs())),
             ('dq', dq[:, :100], ds @ k * scale, e_ds @ k.abs() * scale),
             ('dk', dk, ds.transpose(1, 2) @ q * scale, e_ds.transpose(1, 2) @ q.abs() * scale)):
         excess = (got - want).abs() - bound - u * want.abs() - 2.0 ** -24
