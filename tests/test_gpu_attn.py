@@ -117,6 +117,38 @@ def test_tiles_left_over_after_an_even_share(dtype):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('mask', ['none', 'bool', 'float', 'padding', 'causal'])
+@pytest.mark.parametrize('size', [(1, 530, 8300, 2, 2, 32), (1, 8300, 530, 1, 1, 64), (2, 700, 1500, 2, 1, 128),
+                                  (1, 1100, 1100, 2, 2, 100)], ids=str)
+def test_long_loops_in_parts(size, mask, dtype):
+    # few tiles and long loops: keys (and for dK and dV rows) are split over workgroups and the parts joined
+    say(f'  attention {mask} {size} {dtype}')
+    q, k, v, go, kw = make_attn(size, dtype, mask, seed=3)
+    out, grads = run(q, k, v, go, kw)
+    check_attn(dtype, q, k, v, go, kw, out, grads)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_two_calls_at_once(dtype):
+    # a training step on each of two streams, their kernels and workspaces side by side
+    cases = [make_attn((1, 700, 1500, 2, 1, 128), dtype, 'bool', seed=1), make_attn((2, 300, 900, 4, 4, 32), dtype, 'float')]
+    want = [run(*c[:4], c[4]) for c in cases]
+    inputs = [([t.cuda().requires_grad_() for t in c[:3]], c[3].cuda(), on_gpu(c[4])) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(3):
+        for s, (ts, g, kw) in zip(streams, inputs):
+            with torch.cuda.stream(s):
+                out = td.ma_attn_train(*ts, **kw)
+                got.append((out.detach(),) + torch.autograd.grad(out, ts, g))
+    torch.cuda.synchronize()
+    for i, ts in enumerate(got):
+        for a, b in zip(ts, (want[i % 2][0],) + want[i % 2][1]):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
 def test_a_row_left_nothing_gives_zeros(dtype):
     q, k, v, go, _ = make_attn((2, 40, 50, 2, 2, 32), dtype)
     mask = torch.zeros(2, 1, 40, 50, dtype=torch.bool)
