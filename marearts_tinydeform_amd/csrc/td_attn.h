@@ -33,7 +33,7 @@ struct AttnParams {
     // backward
     const void* go;
     void *dq, *dk, *dv;
-    void* delta;    // [B, H, Q] in the accumulation type: grad_out . out
+    void* delta;    // float64: [B, H, Q], grad_out . out
     // workspace of the forward's key split, of the backward
     void* ws;
 };
@@ -58,8 +58,8 @@ int launch_attn_backward_t(int dtype, const AttnParams& p, hipStream_t stream);
 // Head widths the matrix-unit kernels are built for
 inline int padded_width(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
-// Every launcher returns 0 or a negative TD_E* code after recording a message.
-int launch_attn_forward_generic(int dtype, const AttnParams& p, hipStream_t stream);
-int launch_attn_backward_generic(int dtype, const AttnParams& p, hipStream_t stream);
+// float64 (td_attn.hip). Every launcher returns 0 or a negative TD_E* code after recording a message.
+int launch_attn_forward_f64(const AttnParams& p, hipStream_t stream);
+int launch_attn_backward_f64(const AttnParams& p, hipStream_t stream);
 
 }  // namespace td

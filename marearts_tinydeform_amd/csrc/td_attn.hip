@@ -1,5 +1,5 @@
-// Attention among tokens (include/tinydeform_dense.h): the argument checks of its C entries, and kernels for any type,
-// head width and stride, one wavefront a row, on the vector units.
+// Attention among tokens (include/tinydeform_dense.h): the argument checks of its C entries, float64's kernels, one
+// wavefront a row on the vector units, and masks as bits.
 #include <math.h>
 
 #include "td_attn.h"
@@ -7,12 +7,11 @@
 namespace td {
 namespace {
 
-template <typename T>
-__device__ __forceinline__ const T* at(const void* base, const int64_t (&s)[3], int b, int tok, int h) {
-    return static_cast<const T*>(base) + b * s[0] + static_cast<int64_t>(tok) * s[1] + h * s[2];
+__device__ __forceinline__ const double* at(const void* base, const int64_t (&s)[3], int b, int tok, int h) {
+    return static_cast<const double*>(base) + b * s[0] + static_cast<int64_t>(tok) * s[1] + h * s[2];
 }
 
-constexpr double kLog2eD = 1.4426950408889634;
+constexpr double kLog2eD = 1.4426950408889634, kLowestD = -1.7976931348623157e308;
 
 template <typename A>
 constexpr A neg_inf() {
@@ -20,35 +19,31 @@ constexpr A neg_inf() {
 }
 
 // Whether (query i, key j) is left out by causal, padding or the mask, and the additive mask's term in base 2 (its lowest
-// value kept finite, so that a row of it alone is a uniform row). A -inf of a float mask leaves the pair out whatever its
-// score is.
-template <typename T, typename A>
-__device__ __forceinline__ bool pair_masked(const AttnParams& p, int b, int h, int i, int j, A& add) {
-    add = static_cast<A>(0);
+// value kept finite, so that a row of it alone is a uniform row). A -inf of a float mask leaves the pair out whatever
+// its score is.
+__device__ __forceinline__ bool pair_masked(const AttnParams& p, int b, int h, int i, int j, double& add) {
+    add = 0;
     if (p.causal && j > i + p.diag) return true;
     if (p.pad != nullptr && p.pad[static_cast<int64_t>(b) * p.K + j]) return true;
     if (p.mask_type == TD_MASK_NONE) return false;
     const int64_t m = b * p.ms[0] + h * p.ms[1] + i * p.ms[2] + j;
     if (p.mask_type == TD_MASK_BYTES) return static_cast<const uint8_t*>(p.mask)[m] != 0;
-    add = cvt<A>(static_cast<const T*>(p.mask)[m]);
-    if (add == neg_inf<A>()) return true;
-    const A lowest = static_cast<A>(sizeof(A) == 8 ? -1.7976931348623157e308 : -3.4028234663852886e38);
-    add *= static_cast<A>(kLog2eD);
-    if (add < lowest) add = lowest;
+    add = static_cast<const double*>(p.mask)[m];
+    if (add == neg_inf<double>()) return true;
+    add *= kLog2eD;
+    if (add < kLowestD) add = kLowestD;
     return false;
 }
 
 // scores are in base 2: c = scale * log2(e)
-template <typename A>
-__device__ __forceinline__ A score_factor(const AttnParams& p) {
-    return static_cast<A>(p.scale * kLog2eD);
+__device__ __forceinline__ double score_factor(const AttnParams& p) {
+    return p.scale * kLog2eD;
 }
 
-template <typename A>
-__device__ __forceinline__ A wave_max(A v) {
+__device__ __forceinline__ double wave_max(double v) {
 #pragma unroll
     for (int m = 32; m > 0; m >>= 1) {
-        const A o = xor_lane(v, m);
+        const double o = xor_lane(v, m);
         v = o > v ? o : v;
     }
     return v;
@@ -57,29 +52,28 @@ __device__ __forceinline__ A wave_max(A v) {
 constexpr int kMaxPerLane = TD_ATTN_MAX_HEAD_DIM / kWave;  // head channels per lane
 
 // One wavefront per (b, h, i): keys 64 at a time, one per lane for the scores, then lanes over the head's channels.
-// The running maximum m and sum l (Milakov and Gimelshein's one-pass softmax) are kept in the accumulation type. Bound by
-// the latency of its row loads; the matrix-unit kernels take every case in 16 and 32 bits that they can.
-template <typename T, typename A>
+// The running maximum m and sum l (Milakov and Gimelshein's one-pass softmax) are kept in float64. Bound by the
+// latency of its row loads: float64 is here for checks, not for speed.
 __global__ __launch_bounds__(64) void attn_forward_row_kernel(AttnParams p) {
-    __shared__ A sp[kWave];
+    __shared__ double sp[kWave];
     const int lane = threadIdx.x;
     const int64_t row = blockIdx.x;  // (b * H + h) * Q + i
     const int i = static_cast<int>(row % p.Q), h = static_cast<int>((row / p.Q) % p.H);
     const int b = static_cast<int>(row / p.Q / p.H), hk = h / p.G;
-    const T* q = at<T>(p.q, p.qs, b, i, h);
-    A m = neg_inf<A>(), l = 0, acc[kMaxPerLane] = {};
+    const double* q = at(p.q, p.qs, b, i, h);
+    double m = neg_inf<double>(), l = 0, acc[kMaxPerLane] = {};
     for (int j0 = 0; j0 < p.K; j0 += kWave) {
         const int j = j0 + lane;
-        A t = neg_inf<A>(), add;
-        if (j < p.K && !pair_masked<T, A>(p, b, h, i, j, add)) {
-            const T* k = at<T>(p.k, p.ks, b, j, hk);
-            A s = 0;
-            for (int d = 0; d < p.D; ++d) s += cvt<A>(q[d]) * cvt<A>(k[d]);
-            t = s * score_factor<A>(p) + add;
+        double t = neg_inf<double>(), add;
+        if (j < p.K && !pair_masked(p, b, h, i, j, add)) {
+            const double* k = at(p.k, p.ks, b, j, hk);
+            double s = 0;
+            for (int d = 0; d < p.D; ++d) s += q[d] * k[d];
+            t = s * score_factor(p) + add;
         }
-        const A m_new = wave_max(m > t ? m : t == t ? t : m);
-        const A from = m_new == neg_inf<A>() ? static_cast<A>(0) : m_new;
-        const A shrink = exp2(m - from), e = exp2(t - from);
+        const double m_new = wave_max(m > t ? m : t == t ? t : m);
+        const double from = m_new == neg_inf<double>() ? 0 : m_new;
+        const double shrink = exp2(m - from), e = exp2(t - from);
         m = m_new;
         l = l * shrink + wave_sum(e);
         __syncthreads();
@@ -90,71 +84,68 @@ __global__ __launch_bounds__(64) void attn_forward_row_kernel(AttnParams p) {
         for (int u = 0; u < kMaxPerLane; ++u) {
             const int d = u * kWave + lane;
             if (d >= p.D) break;
-            A o = acc[u] * shrink;
+            double o = acc[u] * shrink;
             for (int x = 0; x < n; ++x)
-                if (sp[x] != 0) o += sp[x] * cvt<A>(at<T>(p.v, p.vs, b, j0 + x, hk)[d]);
+                if (sp[x] != 0) o += sp[x] * at(p.v, p.vs, b, j0 + x, hk)[d];
             acc[u] = o;
         }
     }
-    T* out = static_cast<T*>(p.out) + ((static_cast<int64_t>(b) * p.Q + i) * p.H + h) * p.D;
+    double* out = static_cast<double*>(p.out) + ((static_cast<int64_t>(b) * p.Q + i) * p.H + h) * p.D;
 #pragma unroll
     for (int u = 0; u < kMaxPerLane; ++u) {
         const int d = u * kWave + lane;
-        if (d < p.D) out[d] = static_cast<T>(l == 0 ? static_cast<A>(0) : acc[u] / l);
+        if (d < p.D) out[d] = l == 0 ? 0 : acc[u] / l;
     }
     if (p.stats != nullptr && lane == 0) {
-        A* st = static_cast<A*>(p.stats) + 2 * row;
-        st[0] = l == 0 ? static_cast<A>(0) : m;
-        st[1] = l == 0 ? static_cast<A>(0) : log2(l);
+        double* st = static_cast<double*>(p.stats) + 2 * row;
+        st[0] = l == 0 ? 0 : m;
+        st[1] = l == 0 ? 0 : log2(l);
     }
 }
 
 // delta[row] = grad_out . out of each (b, h, i), one wavefront each
-template <typename T, typename A>
 __global__ __launch_bounds__(64) void attn_delta_row_kernel(AttnParams p) {
     const int lane = threadIdx.x;
     const int64_t row = blockIdx.x;
     const int i = static_cast<int>(row % p.Q), h = static_cast<int>((row / p.Q) % p.H);
     const int64_t at0 = (((row / p.Q / p.H) * p.Q + i) * p.H + h) * p.D;
-    A s = 0;
+    double s = 0;
     for (int d = lane; d < p.D; d += kWave)
-        s += cvt<A>(static_cast<const T*>(p.go)[at0 + d]) * cvt<A>(static_cast<const T*>(p.out)[at0 + d]);
+        s += static_cast<const double*>(p.go)[at0 + d] * static_cast<const double*>(p.out)[at0 + d];
     s = wave_sum(s);
-    if (lane == 0) static_cast<A*>(p.delta)[row] = s;
+    if (lane == 0) static_cast<double*>(p.delta)[row] = s;
 }
 
 // The probability of a pair and the gradient of its score: P = 2^(t - m - log2 l), dS = P (grad_out . v - delta)
-template <typename T, typename A>
-__device__ __forceinline__ void pair_grad(const AttnParams& p, int b, int h, int i, int j, A& prob, A& ds) {
-    A add;
+__device__ __forceinline__ void pair_grad(const AttnParams& p, int b, int h, int i, int j, double& prob, double& ds) {
+    double add;
     prob = ds = 0;
-    if (pair_masked<T, A>(p, b, h, i, j, add)) return;
-    const T* q = at<T>(p.q, p.qs, b, i, h);
-    const T* k = at<T>(p.k, p.ks, b, j, h / p.G);
-    const T* v = at<T>(p.v, p.vs, b, j, h / p.G);
-    const T* g = static_cast<const T*>(p.go) + ((static_cast<int64_t>(b) * p.Q + i) * p.H + h) * p.D;
+    if (pair_masked(p, b, h, i, j, add)) return;
+    const double* q = at(p.q, p.qs, b, i, h);
+    const double* k = at(p.k, p.ks, b, j, h / p.G);
+    const double* v = at(p.v, p.vs, b, j, h / p.G);
+    const double* g = static_cast<const double*>(p.go) + ((static_cast<int64_t>(b) * p.Q + i) * p.H + h) * p.D;
     const int64_t row = (static_cast<int64_t>(b) * p.H + h) * p.Q + i;
-    const A* st = static_cast<const A*>(p.stats) + 2 * row;
-    A s = 0, dp = 0;
+    const double* st = static_cast<const double*>(p.stats) + 2 * row;
+    double s = 0, dp = 0;
     for (int d = 0; d < p.D; ++d) {
-        s += cvt<A>(q[d]) * cvt<A>(k[d]);
-        dp += cvt<A>(g[d]) * cvt<A>(v[d]);
+        s += q[d] * k[d];
+        dp += g[d] * v[d];
     }
-    prob = exp2(s * score_factor<A>(p) + add - st[0] - st[1]);
-    ds = prob * (dp - static_cast<const A*>(p.delta)[row]);
+    prob = exp2(s * score_factor(p) + add - st[0] - st[1]);
+    ds = prob * (dp - static_cast<const double*>(p.delta)[row]);
 }
 
-template <typename T, typename A>
 __global__ __launch_bounds__(64) void attn_dq_row_kernel(AttnParams p) {
-    __shared__ A sd[kWave];
+    __shared__ double sd[kWave];
     const int lane = threadIdx.x;
     const int64_t row = blockIdx.x;
     const int i = static_cast<int>(row % p.Q), h = static_cast<int>((row / p.Q) % p.H);
     const int b = static_cast<int>(row / p.Q / p.H), hk = h / p.G;
-    A acc[kMaxPerLane] = {};
+    double acc[kMaxPerLane] = {};
     for (int j0 = 0; j0 < p.K; j0 += kWave) {
-        A prob = 0, ds = 0;
-        if (j0 + lane < p.K) pair_grad<T, A>(p, b, h, i, j0 + lane, prob, ds);
+        double prob = 0, ds = 0;
+        if (j0 + lane < p.K) pair_grad(p, b, h, i, j0 + lane, prob, ds);
         __syncthreads();
         sd[lane] = ds;
         __syncthreads();
@@ -164,28 +155,27 @@ __global__ __launch_bounds__(64) void attn_dq_row_kernel(AttnParams p) {
             const int d = u * kWave + lane;
             if (d >= p.D) break;
             for (int x = 0; x < n; ++x)
-                if (sd[x] != 0) acc[u] += sd[x] * cvt<A>(at<T>(p.k, p.ks, b, j0 + x, hk)[d]);
+                if (sd[x] != 0) acc[u] += sd[x] * at(p.k, p.ks, b, j0 + x, hk)[d];
         }
     }
-    T* dq = static_cast<T*>(p.dq) + ((static_cast<int64_t>(b) * p.Q + i) * p.H + h) * p.D;
+    double* dq = static_cast<double*>(p.dq) + ((static_cast<int64_t>(b) * p.Q + i) * p.H + h) * p.D;
 #pragma unroll
     for (int u = 0; u < kMaxPerLane; ++u)
-        if (u * kWave + lane < p.D) dq[u * kWave + lane] = static_cast<T>(acc[u] * static_cast<A>(p.scale));
+        if (u * kWave + lane < p.D) dq[u * kWave + lane] = acc[u] * p.scale;
 }
 
 // One wavefront per (b, key head, j): the rows of every head that shares the key, 64 at a time
-template <typename T, typename A>
 __global__ __launch_bounds__(64) void attn_dkv_row_kernel(AttnParams p) {
-    __shared__ A sp[kWave], sd[kWave];
+    __shared__ double sp[kWave], sd[kWave];
     const int lane = threadIdx.x;
     const int64_t id = blockIdx.x;  // (b * Hk + hk) * K + j
     const int j = static_cast<int>(id % p.K), hk = static_cast<int>((id / p.K) % p.Hk);
     const int b = static_cast<int>(id / p.K / p.Hk);
-    A dk[kMaxPerLane] = {}, dv[kMaxPerLane] = {};
+    double dk[kMaxPerLane] = {}, dv[kMaxPerLane] = {};
     for (int r0 = 0; r0 < p.rows; r0 += kWave) {
-        A prob = 0, ds = 0;
+        double prob = 0, ds = 0;
         const int r = r0 + lane;
-        if (r < p.rows) pair_grad<T, A>(p, b, hk * p.G + r % p.G, r / p.G, j, prob, ds);
+        if (r < p.rows) pair_grad(p, b, hk * p.G + r % p.G, r / p.G, j, prob, ds);
         __syncthreads();
         sp[lane] = prob;
         sd[lane] = ds;
@@ -198,9 +188,9 @@ __global__ __launch_bounds__(64) void attn_dkv_row_kernel(AttnParams p) {
             for (int x = 0; x < n; ++x) {
                 const int i = (r0 + x) / p.G, h = hk * p.G + (r0 + x) % p.G;
                 if (sp[x] != 0)
-                    dv[u] += sp[x] * cvt<A>(static_cast<const T*>(
-                                         p.go)[((static_cast<int64_t>(b) * p.Q + i) * p.H + h) * p.D + d]);
-                if (sd[x] != 0) dk[u] += sd[x] * cvt<A>(at<T>(p.q, p.qs, b, i, h)[d]);
+                    dv[u] += sp[x] * static_cast<const double*>(
+                                         p.go)[((static_cast<int64_t>(b) * p.Q + i) * p.H + h) * p.D + d];
+                if (sd[x] != 0) dk[u] += sd[x] * at(p.q, p.qs, b, i, h)[d];
             }
         }
     }
@@ -209,8 +199,8 @@ __global__ __launch_bounds__(64) void attn_dkv_row_kernel(AttnParams p) {
     for (int u = 0; u < kMaxPerLane; ++u) {
         const int d = u * kWave + lane;
         if (d >= p.D) break;
-        static_cast<T*>(p.dk)[o + d] = static_cast<T>(dk[u] * static_cast<A>(p.scale));
-        static_cast<T*>(p.dv)[o + d] = static_cast<T>(dv[u]);
+        static_cast<double*>(p.dk)[o + d] = dk[u] * p.scale;
+        static_cast<double*>(p.dv)[o + d] = dv[u];
     }
 }
 
@@ -219,42 +209,19 @@ int launched(const char* what) {
     return e == hipSuccess ? 0 : set_error(TD_E_LAUNCH, "%s launch failed: %s", what, hipGetErrorString(e));
 }
 
-template <typename T, typename A>
-int forward_row(const AttnParams& p, hipStream_t stream) {
-    hipLaunchKernelGGL((attn_forward_row_kernel<T, A>), dim3(static_cast<unsigned>(p.B) * p.H * p.Q), dim3(64), 0,
-                       stream, p);
+}  // namespace
+
+int launch_attn_forward_f64(const AttnParams& p, hipStream_t stream) {
+    hipLaunchKernelGGL(attn_forward_row_kernel, dim3(static_cast<unsigned>(p.B) * p.H * p.Q), dim3(64), 0, stream, p);
     return launched("attention");
 }
 
-template <typename T, typename A>
-int backward_row(const AttnParams& p, hipStream_t stream) {
+int launch_attn_backward_f64(const AttnParams& p, hipStream_t stream) {
     const unsigned rows = static_cast<unsigned>(p.B) * p.H * p.Q, keys = static_cast<unsigned>(p.B) * p.Hk * p.K;
-    if (rows > 0) hipLaunchKernelGGL((attn_delta_row_kernel<T, A>), dim3(rows), dim3(64), 0, stream, p);
-    if (rows > 0 && p.dq != nullptr)
-        hipLaunchKernelGGL((attn_dq_row_kernel<T, A>), dim3(rows), dim3(64), 0, stream, p);
-    if (keys > 0 && p.dk != nullptr)
-        hipLaunchKernelGGL((attn_dkv_row_kernel<T, A>), dim3(keys), dim3(64), 0, stream, p);
+    if (rows > 0) hipLaunchKernelGGL(attn_delta_row_kernel, dim3(rows), dim3(64), 0, stream, p);
+    if (rows > 0 && p.dq != nullptr) hipLaunchKernelGGL(attn_dq_row_kernel, dim3(rows), dim3(64), 0, stream, p);
+    if (keys > 0 && p.dk != nullptr) hipLaunchKernelGGL(attn_dkv_row_kernel, dim3(keys), dim3(64), 0, stream, p);
     return launched("attention backward");
-}
-
-}  // namespace
-
-int launch_attn_forward_generic(int dtype, const AttnParams& p, hipStream_t stream) {
-    switch (dtype) {
-        case kF32: return forward_row<float, float>(p, stream);
-        case kF16: return forward_row<f16, float>(p, stream);
-        case kBF16: return forward_row<bf16, float>(p, stream);
-        default: return forward_row<double, double>(p, stream);
-    }
-}
-
-int launch_attn_backward_generic(int dtype, const AttnParams& p, hipStream_t stream) {
-    switch (dtype) {
-        case kF32: return backward_row<float, float>(p, stream);
-        case kF16: return backward_row<f16, float>(p, stream);
-        case kBF16: return backward_row<bf16, float>(p, stream);
-        default: return backward_row<double, double>(p, stream);
-    }
 }
 
 namespace {
@@ -457,7 +424,7 @@ extern "C" int td_attn_forward(const td_attn_args* args, void* workspace, int64_
         return set_error(TD_E_WORKSPACE, "attention: the workspace has %lld bytes, %lld are needed",
                          static_cast<long long>(workspace_bytes), static_cast<long long>(need));
     p.ws = workspace;
-    if (args->dtype == TD_F64) return launch_attn_forward_generic(args->dtype, p, static_cast<hipStream_t>(stream));
+    if (args->dtype == TD_F64) return launch_attn_forward_f64(p, static_cast<hipStream_t>(stream));
     return launch_attn_forward(args->dtype, p, static_cast<hipStream_t>(stream));
 }
 
@@ -485,6 +452,6 @@ extern "C" int td_attn_backward(const td_attn_args* args, const void* grad_out, 
     p.dk = grad_key;
     p.dv = grad_value;
     p.ws = p.delta = workspace;
-    if (args->dtype == TD_F64) return launch_attn_backward_generic(args->dtype, p, static_cast<hipStream_t>(stream));
+    if (args->dtype == TD_F64) return launch_attn_backward_f64(p, static_cast<hipStream_t>(stream));
     return launch_attn_backward(args->dtype, p, static_cast<hipStream_t>(stream));
 }
