@@ -55,8 +55,9 @@ int64_t attn_backward_workspace(int dtype, const AttnParams& p);
 int launch_attn_backward(int dtype, const AttnParams& p, hipStream_t stream);
 template <typename T>
 int launch_attn_backward_t(int dtype, const AttnParams& p, hipStream_t stream);
-// Head widths the matrix-unit kernels are built for
-inline int padded_width(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+// Head widths the matrix-unit kernels are built for (80 in 96, 2 x 8 x 4096, bfloat16: forward 168 us in 128, 138 in 96, dQ 219
+// and 170, dK and dV 343 and 240)
+inline int padded_width(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256; }
 
 // float64 (td_attn.hip). Every launcher returns 0 or a negative TD_E* code after recording a message.
 int launch_attn_forward_f64(const AttnParams& p, hipStream_t stream);

@@ -134,10 +134,16 @@ __device__ __forceinline__ float ds_factor(const AttnParams& p, const RowInfo& i
     return __builtin_bit_cast(float, (254u - e) << 23);    // 2^(127 - e)
 }
 
+// Bytes of a row, as the tiles' heights go by them: 32 rows of 192 bytes are no whole number of pieces for 256 threads
+template <typename T, int DP>
+constexpr int staged_bytes() {
+    return DP * static_cast<int>(sizeof(T)) == 192 ? 128 : DP * static_cast<int>(sizeof(T));
+}
+
 // dQ. The forward's shape, WK: private key tiles, the wavefronts' sums joined in LDS.
 template <typename T, int DP, bool WK>
 constexpr int dq_key_tile() {
-    return WK || DP * static_cast<int>(sizeof(T)) > 128 ? 32 : 64;
+    return WK || staged_bytes<T, DP>() > 128 ? 32 : 64;
 }
 // Wavefronts a SIMD that the registers leave room for with few spills or none. A workgroup of eight takes two of each SIMD.
 // dK and dV under a mask (SLOW) stay at two: at four they spill 90 to 120 registers (1100 x 64 heads of 32, bfloat16: 87
@@ -409,7 +415,7 @@ __global__ __launch_bounds__((kWaves<T, DP, WK> * kWave), (dq_min_waves<T, DP, W
 // operands of dV^T = g^T P and dK^T = Q^T dS as they stand. Rows past the end hold zeros and m = inf: P = 0.
 template <typename T, int DP, bool WK>
 constexpr int dkv_row_tile() {
-    return WK || DP * static_cast<int>(sizeof(T)) > 128 ? 32 : 64;
+    return WK || staged_bytes<T, DP>() > 128 ? 32 : 64;
 }
 
 // V of wide heads stays in LDS: its fragments would spill. With dK and dV the registers hold K's fragments only.
@@ -741,15 +747,16 @@ bool back_vec(int dtype, const AttnParams& p) {
 // still leaves CUs without work and the loops are long, parts; where many tiles leave a few over, parts of those
 // (even_split). Measured, both sides: private below 384 x 128 rows (4 key heads x 16000 rows of 64, bfloat16, 500: dQ 170
 // us, shared 143; 2 x 12 heads x 1500, 288: 53, shared 60, dK and dV 67, shared 86), but not for long loops (2 x 8 x 1000 of
-// 32 over 12000 keys: dQ 87, shared 68); a part has 256 steps or more of a shared tile (8 heads x 1500 of 128: dQ 58 us with
-// 512, 44 with 256, dK and dV 87 and 64), 1024 of a private one (3000 rows by 2 x 8 x 200 keys of 64: 33 us, with 512 39,
-// with 256 45); parts below 256 shared workgroups (64 heads x 1100 as 320: dQ 45 us, in parts 52).
+// 32 over 12000 keys: dQ 87, shared 68); a part has 1024 steps or more of a private tile (3000 rows by 2 x 8 x 200 keys of 64:
+// 33 us, with 512 39, with 256 45); parts below 256 shared workgroups (64 heads x 1100 as 320: dQ 45 us, in parts 52).
 BackShape back_shape(int dtype, const AttnParams& p, bool vec) {
     BackShape s{};
     s.vec = vec;
     const int64_t heads = static_cast<int64_t>(p.B) * p.Hk;
     const bool can = vec && padded_width(p.D) * elem_size(dtype) <= 128;
-    auto shape = [&](int n, int over) {
+    const int row_bytes = padded_width(p.D) * elem_size(dtype);
+    // wide: the widest rows of which two workgroups fit on a CU
+    auto shape = [&](int n, int over, int wide) {
         BackShape::One o{};
         const bool long_loop = over >= 8192 && n >= 512;
         o.wk = can && !long_loop && heads * ((n + 127) / 128) < 384;
@@ -757,18 +764,19 @@ BackShape back_shape(int dtype, const AttnParams& p, bool vec) {
         o.tiles = (n + o.tile_rows - 1) / o.tile_rows;
         const int total = static_cast<int>(heads * o.tiles);
         o.t = TileSplit{1, total, total};
-        const int few = o.tile_rows == 256 ? 256 : 384;
-        if (total > 0 && total < few) {
-            const int want = ((o.tile_rows == 256 ? 512 : 1024) + total - 1) / total, most = over / (o.wk ? 1024 : 256);
-            const int parts = want < most ? want : most;
+        if (o.wk && total > 0 && total < 384) {
+            const int want = (1024 + total - 1) / total, most = over / 1024, parts = want < most ? want : most;
+            if (parts > 1) o.t = TileSplit{parts, 0, total};
+        } else if (!o.wk && total > 0 && total < 256) {
+            const int parts = parts_of(total, row_bytes <= wide ? 512 : 256, over, dtype == kF32);
             if (parts > 1) o.t = TileSplit{parts, 0, total};
         } else if (!o.wk && !p.causal) {
             o.t = even_split(total, (over + 63) / 64);
         }
         return o;
     };
-    s.q = shape(p.rows, p.K);
-    s.k = shape(p.K, p.rows);
+    s.q = shape(p.rows, p.K, 128);
+    s.k = shape(p.K, p.rows, 64);
     return s;
 }
 
@@ -880,6 +888,7 @@ int launch_attn_backward_t(int dtype, const AttnParams& given, hipStream_t strea
     switch (padded_width(p.D)) {
         case 32: rc = run_dp<T, 32>(p, s, info, ws, stream); break;
         case 64: rc = run_dp<T, 64>(p, s, info, ws, stream); break;
+        case 96: rc = run_dp<T, 96>(p, s, info, ws, stream); break;
         case 128: rc = run_dp<T, 128>(p, s, info, ws, stream); break;
         default: rc = run_dp<T, 256>(p, s, info, ws, stream);
     }

@@ -36,7 +36,7 @@ __device__ __forceinline__ float shift_of(float m) {
 
 struct Split {
     TileSplit t;
-    int keys;   // keys of a part, a multiple of 256
+    int keys;   // keys of a part, a multiple of 128
     float* o;   // parts' unnormalised outputs [..][rows of a tile][D]
     float* ml;  // and maximum and sum [..][rows of a tile][2]
 };
@@ -416,18 +416,20 @@ Shape shape_of(int dtype, const AttnParams& p) {
     s.tiles = (p.rows + s.tile_rows - 1) / s.tile_rows;
     const int total = static_cast<int>(heads * s.tiles);
     s.t = TileSplit{1, total, total};
-    const bool big = s.tile_rows == 256;                  // of 512 threads: two such workgroups fill a CU
-    if (total < (big || s.wk ? 256 : 512) && p.K > 1024) {
-        int64_t n = ((big ? 512 : 1024) + total - 1) / total;
+    if (s.wk && total < 256 && p.K > 1024) {
+        int64_t n = (1024 + total - 1) / total;
         const int64_t most = (p.K + 511) / 512;
         n = n < most ? n : most;
         n = n < kJoinParts ? n : kJoinParts;
-        s.t = TileSplit{static_cast<int>(n), n > 1 ? 0 : total, total};
+        s.t = TileSplit{static_cast<int>(n), 0, total};
+    } else if (!s.wk && total < 256) {
+        const int n = parts_of(total, padded_width(p.D) * elem <= 128 ? 512 : 256, p.K, dtype == kF32);
+        s.t = TileSplit{n, n > 1 ? 0 : total, total};
     } else if (!s.wk && !p.causal) {  // causal tiles differ in length and even out by themselves
         s.t = even_split(total, (p.K + 63) / 64);
     }
-    const int64_t keys = ((p.K + s.t.n - 1) / s.t.n + 255) / 256 * 256;
-    s.keys = static_cast<int>(keys < 2147483392 ? keys : 2147483392);
+    const int64_t keys = ((p.K + s.t.n - 1) / s.t.n + 127) / 128 * 128;
+    s.keys = static_cast<int>(keys < 2147483520 ? keys : 2147483520);
     return s;
 }
 
@@ -487,6 +489,7 @@ int launch_attn_forward_t(int dtype, const AttnParams& p, hipStream_t stream) {
     switch (padded_width(p.D)) {
         case 32: return run_dp<T, 32>(q, s, sp, stream);
         case 64: return run_dp<T, 64>(q, s, sp, stream);
+        case 96: return run_dp<T, 96>(q, s, sp, stream);
         case 128: return run_dp<T, 128>(q, s, sp, stream);
         default: return run_dp<T, 256>(q, s, sp, stream);
     }
