@@ -298,7 +298,7 @@ inline TileSplit even_split(int total, int steps) {
 // tiles on 512 slots: 20 whole, 29 in 3.
 inline int parts_of(int total, int slots, int64_t loop, bool float32) {
     const double steps = loop / 64.0, fixed = float32 ? 1 : 4;
-    const int64_t most = loop / 128 < 1024 ? loop / 128 : 1024;
+    const int64_t most = loop < 131072 ? (loop + 127) / 128 : 1024;
     int best = 1;
     double least = (total + slots - 1) / slots * (steps + fixed);
     for (int64_t rounds = 1; rounds <= 4; ++rounds) {
